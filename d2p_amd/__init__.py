@@ -6,6 +6,9 @@ order: the same Python API (``soft_sw``, ``soft_sw_affine``, ``soft_dtw``,
 ``soft_nw``, ``soft_nw_affine``, the ``nn.Module`` wrappers, ``ops``, the legacy flat
 names) and the same ``torch.ops.d2p`` operator schemas, computed by hand-written HIP
 kernels for CDNA4.  Tensors must live on the HIP device.
+
+Beside it stand the operators of the sequence encoders that make the scores' embeddings
+(``attention``, ``qk_norm_rope``, ``SequenceAttention``), which the reference does not have.
 """
 from . import _ops
 from . import _compile  # noqa: F401  (fake/meta and autocast registrations)
@@ -13,6 +16,8 @@ from . import _compile  # noqa: F401  (fake/meta and autocast registrations)
 from .sw import soft_sw, soft_sw_affine, SWResult, SoftSW, SoftSWAffine
 from .dtw import soft_dtw, soft_dtw_sqeuclidean, DTWResult, SoftDTW
 from .nw import soft_nw, soft_nw_affine, NWResult, SoftNW, SoftNWAffine
+from .encoder import (attention, qk_norm_rope, relative_buckets, rope_tables, KeyValueCache,
+                      SequenceAttention)
 from . import ops
 
 # legacy flat names (reference d2p/__init__.py:120-139)
@@ -56,4 +61,6 @@ __all__ = [
     "soft_nw_hvp", "soft_nw_param_jacobian", "soft_nw_backward_full",
     "soft_nw_affine", "SoftNWAffine", "soft_nw_affine_float", "soft_nw_affine_with_grads",
     "soft_nw_affine_hvp", "soft_nw_affine_param_jacobian", "soft_nw_affine_backward_full",
+    "attention", "qk_norm_rope", "relative_buckets", "rope_tables", "KeyValueCache",
+    "SequenceAttention",
 ]

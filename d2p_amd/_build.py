@@ -2,9 +2,9 @@
 
 * ``libd2p_amd.so`` -- the HIP kernels for gfx950 and their C ABI
   (``include/d2p_amd.h``), compiled with hipcc;
-* ``_C.so``         -- the PyTorch operator layer (``csrc/torch_ops.cpp``),
-  compiled with g++ against the installed torch and linked to libd2p_amd.so
-  through an ``$ORIGIN`` rpath.
+* ``_C.so``         -- the PyTorch operator layer (``csrc/*.cpp``), compiled with
+  g++ against the installed torch and linked to libd2p_amd.so through an
+  ``$ORIGIN`` rpath.
 
 Both land next to this file so they travel with the source tree.
 """
@@ -68,18 +68,26 @@ def build_ops() -> str:
     tinc = os.path.join(tdir, "include")
     tlib = os.path.join(tdir, "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    tmp = OP_LIB + ".tmp"
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+    flags = [
+        "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-w",
         f"-I{tinc}", f"-I{os.path.join(tinc, 'torch', 'csrc', 'api', 'include')}",
         f"-I{os.path.join(ROCM, 'include')}", f"-I{INCLUDE}",
-        src, "-o", tmp,
-        f"-L{PKG}", "-ld2p_amd", f"-L{tlib}", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
-        "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}",
     ]
-    _run(cmd)
+
+    def compile_cpp(src: str) -> str:
+        obj = os.path.join(OBJ, os.path.basename(src) + ".o")
+        _run(["g++", *flags, "-c", src, "-o", obj])
+        return obj
+
+    os.makedirs(OBJ, exist_ok=True)
+    srcs = sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
+    with cf.ThreadPoolExecutor(max_workers=max(1, len(srcs))) as ex:
+        objs = list(ex.map(compile_cpp, srcs))
+    tmp = OP_LIB + ".tmp"
+    _run(["g++", "-shared", *objs, "-o", tmp,
+          f"-L{PKG}", "-ld2p_amd", f"-L{tlib}", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
+          "-lc10", "-lc10_hip", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"])
     os.replace(tmp, OP_LIB)
     return OP_LIB
 

@@ -113,6 +113,30 @@ _AMD_FAKES = {
 for _name, _fn in _AMD_FAKES.items():
     register_fake(f"d2p_amd::{_name}")(_fn)
 
+
+# the sequence-encoder operators: contiguous results; their autocast rule is their own
+def _contiguous(x):
+    return x.new_empty(x.shape)
+
+
+def _stats(q):
+    return q.new_empty([2, q.size(0), q.size(2), q.size(1)], dtype=torch.float32)
+
+
+_ENCODER_FAKES = {
+    "attention": lambda q, k, v, *options: _contiguous(q),
+    "attention_forward": lambda q, k, v, *options: (_contiguous(q), _stats(q)),
+    "attention_backward": lambda grad, q, k, v, out, stats, l, causal, scale, bias, buckets, p,
+    seed, seed_tensor, bias_grad: (_contiguous(q), _contiguous(k), _contiguous(v),
+                                   _contiguous(bias) if bias_grad else q.new_empty([0])),
+    "qk_norm_rope": lambda q, k, *options: (_contiguous(q), _contiguous(k)),
+    "qk_norm_rope_backward": lambda gq, gk, q, k, wq, wk, cos, sin, pos, eps, interleaved, w: (
+        _contiguous(q), _contiguous(k),
+        *(q.new_empty([q.size(3) if w else 0], dtype=torch.float32) for _ in range(2))),
+}
+for _name, _fn in _ENCODER_FAKES.items():
+    register_fake(f"d2p_amd::{_name}")(_fn)
+
 try:
     from torch.library import register_autocast
 except ImportError:  # older torch: autocast rules unavailable

@@ -11,18 +11,13 @@
 // libd2p_amd.so on the current HIP stream.  There is no CPU implementation: CPU
 // tensors raise.
 
-#include <torch/torch.h>
-#include <torch/library.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-
 #include <cstdlib>
 #include <cstring>
 #include <limits>
 #include <tuple>
 #include <vector>
 
-#include "../../include/d2p_amd.h"
+#include "torch_util.h"
 
 namespace {
 
@@ -30,22 +25,12 @@ using torch::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::tensor_list;
 
-#define D2P_CALL(expr)                                                          \
-    do {                                                                        \
-        int rc_ = (expr);                                                       \
-        TORCH_CHECK(rc_ == 0, "d2p_amd kernel call failed: ", d2p_last_error()); \
-    } while (0)
-
 // same wording as /root/reference/src/common/torch_utils.h:31-66
 #define CHECK_INPUT_DEV(x)                                                      \
     TORCH_CHECK((x).is_cuda(), #x " must be a CUDA tensor");                   \
     TORCH_CHECK((x).is_contiguous(), #x " must be contiguous");                \
     TORCH_CHECK((x).scalar_type() == torch::kFloat32, #x " must be float32, got ", \
                 (x).scalar_type())
-
-inline void* current_stream() {
-    return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
-}
 
 struct Dims {
     int B, L1, L2;
@@ -154,11 +139,6 @@ const int* lengths_ptr(const Tensor& lengths) {
 // (an undefined Tensor input has no device for the autograd node to record).
 c10::optional<Tensor> lengths_arg(const Tensor& lengths) {
     return lengths.defined() ? c10::optional<Tensor>(lengths) : c10::nullopt;
-}
-
-Tensor workspace(size_t bytes, const Tensor& like) {
-    return torch::empty({(int64_t)std::max<size_t>(bytes, 1)},
-                        like.options().dtype(torch::kUInt8));
 }
 
 float scalar_value(const Tensor& t, const char* name) {
@@ -1219,12 +1199,6 @@ std::tuple<Tensor, Tensor> dtw_backward_full(Tensor costs, Tensor grad_alignment
     return {std::get<0>(r), std::get<1>(r).sum().reshape({1})};
 }
 
-[[noreturn]] void cpu_unsupported() {
-    TORCH_CHECK(false,
-                "d2p_amd implements the MI355X (HIP) path only: move the inputs to a "
-                "HIP device (device='cuda' on PyTorch-ROCm)");
-}
-
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -1478,7 +1452,6 @@ TORCH_LIBRARY_IMPL(d2p, AutogradCUDA, m) {
 }
 
 namespace {
-void cpu_boxed(const c10::OperatorHandle&, torch::jit::Stack*) { cpu_unsupported(); }
 const char* const kAllOps[] = {
     "soft_sw", "soft_sw_float", "soft_sw_with_grads", "soft_sw_hvp", "soft_sw_param_jacobian",
     "soft_sw_backward_full", "sw_forward", "sw_forward_t", "sw_value_grad_params",
