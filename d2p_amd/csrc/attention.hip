@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "attention_backward.hip.h"
+#include "attention_few.hip.h"
 
 namespace d2p_amd {
 namespace enc {
@@ -72,8 +73,8 @@ using namespace d2p_amd;
 using namespace d2p_amd::enc;
 
 extern "C" size_t d2p_attention_workspace_bytes(const d2p_attention_params* p) {
-    (void)p;
-    return 0;
+    FewPlan pl;
+    return p && check_attention(p) == D2P_OK && plan_few(*p, &pl) ? few_floats(*p, pl) * 4 : 0;
 }
 
 extern "C" int d2p_attention_forward(const d2p_attention_params* p, const void* q, const void* k,
@@ -84,10 +85,21 @@ extern "C" int d2p_attention_forward(const d2p_attention_params* p, const void* 
     D2P_REQUIRE(q && out && stats && ((k && v) || p->Lk == 0), "null pointer argument");
     D2P_REQUIRE(aligned(q) && aligned(k) && aligned(v) && aligned(out),
                 "tensors must be aligned to 16 bytes");
-    (void)workspace;
-    (void)workspace_bytes;
     const ForwardArgs a{*p, q, k, v, out, stats};
     hipStream_t st = (hipStream_t)stream;
+    FewArgs few{a};
+    if (plan_few(*p, &few.plan)) {
+        const size_t floats = few_floats(*p, few.plan);
+        D2P_REQUIRE(floats == 0 || (workspace && workspace_bytes >= floats * 4),
+                    "workspace too small");
+        const size_t rows = (size_t)p->B * p->Hkv * few.plan.rows * few.plan.parts;
+        few.acc = (float*)workspace;
+        few.part_m = few.acc + rows * p->D;
+        few.part_l = few.part_m + rows;
+        return p->dtype == D2P_FLOAT32   ? launch_few_f32(few, st)
+               : p->dtype == D2P_FLOAT16 ? launch_few_f16(few, st)
+                                         : launch_few_bf16(few, st);
+    }
     return p->dtype == D2P_FLOAT32   ? launch_forward_f32(a, st)
            : p->dtype == D2P_FLOAT16 ? launch_forward_f16(a, st)
                                      : launch_forward_bf16(a, st);

@@ -354,8 +354,14 @@ __device__ __forceinline__ Rows head_rows(const void* x, const d2p_strides& s, i
                 D / Elem<T>::PER};
 }
 
+// A bias in units of log2; a finite one stays finite.
+__device__ __forceinline__ float in_log2(float v) {
+    const float big = 3.4028235e38f;
+    return v >= -big && v <= big ? fminf(fmaxf(v * LOG2E, -big), big) : v;
+}
+
 // The bias of each clipped distance for head h, in units of log2: bias[0 .. 2 R] in LDS.
-// -inf masks a pair; a finite entry stays finite.
+// -inf masks a pair.
 template <class T>
 __device__ __forceinline__ void load_bias(float* lds, const d2p_attention_params& p, int h,
                                           int tid, int threads) {
@@ -365,8 +371,7 @@ __device__ __forceinline__ void load_bias(float* lds, const d2p_attention_params
         if (n >= 0 && n < p.num_buckets) {
             const long long i = (long long)n * p.Hq + h;
             v = p.bias_dtype == D2P_FLOAT32 ? ((const float*)p.bias)[i] : Elem<T>::load(p.bias, i);
-            const float big = 3.4028235e38f;
-            if (v >= -big && v <= big) v = fminf(fmaxf(v * LOG2E, -big), big);
+            v = in_log2(v);
         }
         lds[t] = v;
     }
