@@ -6,6 +6,8 @@
 // fixed order.  A wave keeps one tile of 32 keys in flight while it works on another: K in
 // the registers that the matrix cores read, V through registers to its own part of LDS.
 #pragma once
+#include <cmath>
+
 #include "attention_forward.hip.h"
 
 namespace d2p_amd {
@@ -281,13 +283,27 @@ __global__ void __launch_bounds__(256) attention_join_kernel(FewArgs fa) {
 }
 
 // Whether a call goes this way, and how it is cut.
+//
+// Both ways' times in us, from what they measured on 256 compute units.  attention_forward
+// passes over all keys with each of its blocks of 128 queries: 0.8 to 1 us for each 64 keys
+// and each block that a compute unit gets.  This way costs 55 keys (of 128 features) a us and
+// compute unit for each tile of 32 rows, and the join 1 us for each 1000 rows.  Measured, one
+// way / the other (16 batch elements, 8 key heads of 128, 2048 keys, 4 query heads each): 1 query
+// 67 / 37 us, 16 queries 66 / 59, 32 queries 64 / 78; 2 heads over 16384 keys: 1 query 263 / 15,
+// 256 queries 267 / 38; 32 heads of 8 over 1024 keys, 128 queries: 23 / 28.
 inline bool plan_few(const d2p_attention_params& p, FewPlan* pl) {
     if (p.drop || p.B == 0 || p.Lq == 0) return false;
-    const int cus = device_cus() > 0 ? device_cus() : 256;
-    const long long blocks = (long long)p.B * p.Hq * cdiv(p.Lq, 128);
-    if (p.Lq > 16 && !(2 * blocks <= cus && p.Lk >= 1024)) return false;
+    const int cus = device_cus() > 0 ? device_cus() : 256, dp = padded(p.D);
+    const bool wide = p.dtype == D2P_FLOAT32;
     const long long rows = (long long)p.Hq / p.Hkv * p.Lq;
     if (rows > 1 << 20) return false;
+    const double all = (double)p.B * p.Hq * p.Lq;
+    const double blocks = (double)p.B * p.Hq * cdiv(p.Lq, 128);
+    const double forward = std::ceil(blocks / cus) * cdiv(p.Lk, 64) *
+                           (wide ? dp / 12.8 : 0.6 + dp / 320.0);
+    const double few = 3 + all / 1000 + (double)p.B * p.Hkv * cdiv((int)rows, 32) * p.Lk /
+                       (cus * (wide ? 3264.0 : 7040.0) / dp);
+    if (few > forward) return false;
     pl->rows = (int)rows;
     pl->row_tiles = cdiv(pl->rows, 32);
     const long long base = (long long)p.B * p.Hkv * pl->row_tiles;

@@ -3,6 +3,13 @@
 // Scores are formed transposed, S^T = K Q^T, so that a lane holds one query and 16 keys of
 // each 32: its softmax is lane-local but for one exchange of the two half waves, and P^T
 // is the second operand of O^T = V^T P^T as it stands (encoder.hip.h).
+//
+// Bound, for 64 keys and 32 queries of 128 features of 16 bits: 32 MFMAs of 32 cycles against
+// 64 exponentials (16 cycles a wave) and about 100 other vector operations (4 cycles) a lane,
+// near 1000 cycles each on a SIMD, and 32 KiB of LDS reads for the wave, which four SIMDs'
+// matrix cores would take in those 1000 cycles too.  Two waves a SIMD, one's exponentials
+// beside the other's products; accumulators in architectural registers (256 a wave), where
+// the vector units read them without a copy.
 #pragma once
 #include "encoder.hip.h"
 
@@ -44,155 +51,282 @@ __device__ __forceinline__ int bias_reach(int j0, int j1, int at0, int R) {
     return j1 - at0 <= -R ? -1 : j0 - (at0 + 31) >= R ? 1 : 0;
 }
 
-// A workgroup takes 128 queries of one head, 32 a wave, and passes over the keys 64 at a
-// time: K and V tiles through registers to LDS, one tile ahead.
-template <class T, int DP, bool BIAS, bool DROP>
-__global__ void __launch_bounds__(256) attention_forward_kernel(ForwardArgs a) {
+// Shared by the waves of a workgroup: K and V tiles of 64 keys, two of each, which go to
+// LDS without passing through registers while the tiles before them are worked on.
+//
+// A wave takes QT tiles of 32 queries.  In one turn of its loop the matrix cores form the
+// next tile's scores while its vector units take the exponentials of this one, and P V of
+// each half of the keys while they take those of the other half and the next maximum.  The
+// accumulators are scaled to a new maximum only when it has grown by more than 2^8 (a
+// branch that is soon rare); until then the old one is a reference as good.
+template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward {
     using TL = Tile<T, DP>;
-    constexpr int BK = 64, DT = DP / 32;
+    using E = Elem<T>;
+    static constexpr int BK = 64, DT = DP / 32, TILE = TL::bytes(BK) / 16;
+    static constexpr int LDS = 4 * TL::bytes(BK);   // and the bias's table
+
+    const ForwardArgs& a;
+    const d2p_attention_params& p;
+    const u4v* Ks;
+    const u4v* Vs;
+    const float* bias;
+    const Drop drop;
+    int lane, h, wq, at0;
+    int at[QT], limit[QT];
+    u4v qf[QT][TL::STEPS];
+    f16v o[QT][DT] = {};
+    float m[QT], ref[QT], l[QT];
+    float c;
+
+    __device__ __forceinline__ Forward(const ForwardArgs& a_, const Span& e, const Rows& qr,
+                                       const u4v* sm, const float* bias_, int bh, int wq_,
+                                       int lane_)
+        : a(a_), p(a_.p), Ks(sm), Vs(sm + 2 * TILE), bias(bias_), drop(a_.p, bh), lane(lane_),
+          h(lane_ >> 5), wq(wq_), at0(wq_ + e.off) {
+        c = p.scale * LOG2E;
+        const __amdgpu_buffer_rsrc_t r = qr.from(wq);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int i = wq + 32 * t + (lane & 31);
+            at[t] = i + e.off;
+            limit[t] = e.limit(p, i);
+            m[t] = -__builtin_inff();
+            ref[t] = 0.0f;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < TL::STEPS; ++s)
+                qf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(r, qr.at(i - wq, 2 * s + h), 0, 0);
+        }
+    }
+
+    __device__ __forceinline__ void scores(f16v (&s)[2][QT], int buf) const {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t) s[k][t] = f16v{};
+#pragma unroll
+            for (int n = 0; n < TL::STEPS; ++n) {
+                const u4v kf = TL::frag(Ks + buf * TILE, 32 * k, n, lane);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) s[k][t] = E::mma(kf, qf[t][n], s[k][t]);
+            }
+        }
+    }
+
+    // Bias and mask of the tile from key j0 on, and its place against the reference.
+    __device__ __forceinline__ void settle(f16v (&s)[2][QT], int j0, bool full) {
+        const int R = p.max_distance;
+        const float inf = __builtin_inff();
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                if (BIAS) {
+                    const int j = j0 + 32 * k, far = bias_reach(j, j + 31, at0 + 32 * t, R);
+                    if (far) {
+                        const float b = bias[far < 0 ? 0 : 2 * R];
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) s[k][t][v] = fmaf(s[k][t][v], c, b);
+                    } else {
+                        const int d = j + 4 * h - at[t];
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            const int n = d + 8 * (v >> 2) + (v & 3);
+                            s[k][t][v] = fmaf(s[k][t][v], c, bias[min(max(n, -R), R) + R]);
+                        }
+                    }
+                }
+                if (!full) {
+                    const int left = limit[t] - (j0 + 32 * k + 4 * h);
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        s[k][t][v] = 8 * (v >> 2) + (v & 3) < left ? s[k][t][v] : -inf;
+                }
+            }
+        bool grown = false;
+        float top[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            float x = s[0][t][0];
+#pragma unroll
+            for (int v = 1; v < 32; ++v) x = fmaxf(x, s[v >> 4][t][v & 15]);
+            top[t] = both_max(x) * (BIAS ? 1.0f : c);
+            grown |= top[t] > m[t] + 8.0f;
+        }
+        if (__any(grown)) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float to = fmaxf(m[t], top[t]);
+                const float f = to > m[t] ? exp2_(m[t] - to) : 1.0f;   // 0 from -inf
+                m[t] = to;
+                ref[t] = to == -inf ? 0.0f : to - FORWARD_SHIFT<T>;
+                l[t] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[t][d] *= f;
+            }
+        }
+    }
+
+    // exponentials of half k of a tile: P, ready for the matrix cores
+    __device__ __forceinline__ void weights(const f16v (&s)[2][QT], int k, int j0,
+                                            u4v (&pf)[QT][TL::FRAGS]) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            float x[16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                x[v] = exp2_(BIAS ? s[k][t][v] - ref[t] : fmaf(s[k][t][v], c, -ref[t]));
+                l[t] += x[v];
+            }
+            if (DROP) {
+                const u4v kw = drop.by_query(wq + 32 * t, j0 + 32 * k, lane);
+#pragma unroll
+                for (int v = 0; v < 16; ++v) x[v] = drop.keeps(kw, v) ? x[v] : 0.0f;
+            }
+            // P in the type of V: its rounding is that of one factor of each product
+#pragma unroll
+            for (int f = 0; f < TL::FRAGS; ++f) pf[t][f] = E::pack(x + TL::PER * f);
+        }
+    }
+
+    __device__ __forceinline__ void values(const u4v (&pf)[QT][TL::FRAGS], int k, int buf) {
+#pragma unroll
+        for (int f = 0; f < TL::FRAGS; ++f)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const u4v vf = TL::frag_t(Vs + buf * TILE, 32 * k, 32 * d, f, lane);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) o[t][d] = E::mma(vf, pf[t][f], o[t][d]);
+            }
+    }
+
+    __device__ __forceinline__ void store(const Span& e, int b, int hq, int bh) {
+        const int D = p.D;
+        const float nan = __builtin_nanf("");
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int i = wq + 32 * t + (lane & 31);
+            const float sum = both_sum(l[t]);
+            if (i >= p.Lq) continue;
+            // no key: zeros, whatever the accumulators hold
+            const bool none = i >= e.nq || !(sum != 0.0f);
+            const float f = (DROP ? drop.scale : 1.0f) / sum;
+            char* row = (char*)a.out +
+                        (((long long)b * p.Lq + i) * p.Hq + hq) * D * (long long)sizeof(T);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d0 = 32 * d + 8 * g + 4 * h;
+                    float y[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        y[r] = e.bad ? nan : none ? 0.0f : o[t][d][4 * g + r] * f;
+                    if (d0 < D) E::store4(row + d0 * (int)sizeof(T), y);
+                }
+            if (h == 0) {
+                const long long n = (long long)p.B * p.Hq * p.Lq, x = (long long)bh * p.Lq + i;
+                a.stats[x] = e.bad ? nan : none ? -__builtin_inff() : m[t];
+                a.stats[n + x] = none ? 0.0f : log2_(sum) - FORWARD_SHIFT<T>;
+            }
+        }
+    }
+};
+
+template <class T, int DP, int QT, int NW, bool BIAS, bool DROP>
+__global__ void __launch_bounds__(64 * NW, sizeof(T) * DP >= 512 ? 1 : 2)
+attention_forward_kernel(ForwardArgs a) {
+    using F = Forward<T, DP, QT, NW, BIAS, DROP>;
+    using TL = Tile<T, DP>;
+    constexpr int BK = F::BK, ROWS = 32 * QT * NW;
     extern __shared__ __align__(16) u4v sm[];
     u4v* Ks = sm;
-    u4v* Vs = Ks + TL::bytes(BK) / 16;
-    float* bias = (float*)(Vs + TL::bytes(BK) / 16);
+    u4v* Vs = sm + 2 * F::TILE;
+    float* bias = (float*)(sm + 4 * F::TILE);
     const d2p_attention_params& p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int nb = (p.Lq + 127) / 128;
-    const unsigned w = near_xcd(blockIdx.x, gridDim.x);
-    const int bh = w / nb, b = bh / p.Hq, hq = bh % p.Hq;
-    // causal: the blocks with the most keys first
-    const int q0 = (p.causal ? nb - 1 - (int)(w % nb) : (int)(w % nb)) * 128;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int nb = (p.Lq + ROWS - 1) / ROWS;
+    int bh, block;
+    place(blockIdx.x, p.B * p.Hq, nb, p.causal, &bh, &block);
+    const int b = bh / p.Hq, hq = bh % p.Hq, hk = hq / (p.Hq / p.Hkv);
+    const int q0 = (p.causal ? nb - 1 - block : block) * ROWS;   // the most keys first
     const Span e(p, b);
-    const int D = p.D, wq = q0 + 32 * wave, i = wq + (lane & 31), at = i + e.off;
-    const Rows qr = head_rows<T>(a.q, p.q, b, hq, e.nq, D);
-    const Rows kr = head_rows<T>(a.k, p.k, b, hq / (p.Hq / p.Hkv), e.nk, D);
-    const Rows vr = head_rows<T>(a.v, p.v, b, hq / (p.Hq / p.Hkv), e.nk, D);
-    if (BIAS) load_bias<T>(bias, p, hq, tid, 256);
+    const Rows qr = head_rows<T>(a.q, p.q, b, hq, e.nq, p.D);
+    const Rows kr = head_rows<T>(a.k, p.k, b, hk, e.nk, p.D);
+    const Rows vr = head_rows<T>(a.v, p.v, b, hk, e.nk, p.D);
+    // keys that the block's last query sees, in tiles
+    const int end = q0 < e.nq ? e.limit(p, min(q0 + ROWS, e.nq) - 1) : 0;
+    const int tiles = (end + BK - 1) / BK;
 
-    u4v qf[TL::STEPS];
-    {
-        const __amdgpu_buffer_rsrc_t r = qr.from(q0);
-#pragma unroll
-        for (int s = 0; s < TL::STEPS; ++s)
-            qf[s] = __builtin_amdgcn_raw_buffer_load_b128(r, qr.at(i - q0, 2 * s + h), 0, 0);
-    }
-    const float c = p.scale * LOG2E;
-    const Drop drop(p, bh);
-    f16v o[DT] = {};
-    float m = -__builtin_inff(), l = 0.0f;
-    // keys that the block's, the wave's first and the lane's query see
-    const int end = q0 < e.nq ? e.limit(p, min(q0 + 127, e.nq - 1)) : 0;
-    const int wave_full = e.limit(p, wq);
-    const int limit = e.limit(p, i);
-
-    Stage<T, DP, BK, 256> ks, vs;
-    if (end > 0) {
-        ks.load(kr, 0, tid);
-        vs.load(vr, 0, tid);
-    }
-    for (int j0 = 0; j0 < end; j0 += BK) {
+    TileDma<T, DP, BK, NW> dk, dv;
+    dk.init(kr, wave, lane);
+    dv.init(vr, wave, lane);
+    if (tiles > 0) dk.issue(kr, 0, Ks, wave);
+    if (BIAS) load_bias<T>(bias, p, hq, tid, 64 * NW);
+    F f(a, e, qr, sm, bias, bh, q0 + 32 * QT * wave, lane);
+    const int wave_full = e.limit(p, f.wq);   // keys that all of the wave's queries see
+    if (tiles > 0) {
+        f16v s0[2][QT], s1[2][QT];
+        wait_dma();
         __syncthreads();
-        ks.store(Ks, tid);
-        vs.store(Vs, tid);
-        __syncthreads();
-        if (j0 + BK < end) {
-            ks.load(kr, j0 + BK, tid);
-            vs.load(vr, j0 + BK, tid);
-        }
-        float x[32];
-        const int far = BIAS ? bias_reach(j0, j0 + BK - 1, wq + e.off, p.max_distance) : 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f16v s = {};
-#pragma unroll
-            for (int n = 0; n < TL::STEPS; ++n)
-                s = Elem<T>::mma(TL::frag(Ks, 32 * t, n, lane), qf[n], s);
-            if (j0 + BK <= wave_full)
-                score_tile<BIAS, true>(s, c, bias, p.max_distance, far, j0 + 32 * t, at, limit,
-                                       lane, x + 16 * t);
-            else
-                score_tile<BIAS, false>(s, c, bias, p.max_distance, far, j0 + 32 * t, at, limit,
-                                        lane, x + 16 * t);
-        }
-        float top = x[0];
-#pragma unroll
-        for (int v = 1; v < 32; ++v) top = fmaxf(top, x[v]);
-        top = fmaxf(m, both_max(top));
-        const float ref = (top == -__builtin_inff() ? 0.0f : top) - FORWARD_SHIFT<T>;
-        const float old = exp2_(m - (FORWARD_SHIFT<T> + ref));   // nothing seen yet: 0
-        m = top;
-        l *= old;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= old;
-#pragma unroll
-        for (int v = 0; v < 32; ++v) {
-            x[v] = exp2_(x[v] - ref);
-            l += x[v];
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            if (DROP) {
-                const u4v kw = drop.by_query(wq, j0 + 32 * t, lane);
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    x[16 * t + v] = drop.keeps(kw, v) ? x[16 * t + v] : 0.0f;
-            }
-#pragma unroll
-            for (int f = 0; f < TL::FRAGS; ++f) {
-                // P in the type of V: its rounding is that of one factor of each product
-                const u4v pf = Elem<T>::pack(x + 16 * t + TL::PER * f);
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    o[d] = Elem<T>::mma(TL::frag_t(Vs, 32 * t, 32 * d, f, lane), pf, o[d]);
-            }
+        dv.issue(vr, 0, Vs, wave);
+        if (tiles > 1) dk.issue(kr, BK, Ks + F::TILE, wave);
+        f.scores(s0, 0);
+        f.settle(s0, 0, BK <= wave_full);
+        auto turn = [&](f16v (&now)[2][QT], f16v (&next)[2][QT], int n, int buf) {
+            wait_dma();
+            meet();
+            if (n + 1 < tiles) dv.issue(vr, (n + 1) * BK, Vs + (buf ^ 1) * F::TILE, wave);
+            if (n + 2 < tiles) dk.issue(kr, (n + 2) * BK, Ks + buf * F::TILE, wave);
+            u4v p0[QT][TL::FRAGS], p1[QT][TL::FRAGS];
+            f.scores(next, buf ^ 1);   // past the last tile: of no use, and harmless
+            f.weights(now, 0, n * BK, p0);
+            f.values(p0, 0, buf);
+            f.weights(now, 1, n * BK, p1);
+            f.values(p1, 1, buf);
+            if (n + 1 < tiles) f.settle(next, (n + 1) * BK, (n + 2) * BK <= wave_full);
+        };
+        for (int n = 0; n < tiles; n += 2) {
+            turn(s0, s1, n, 0);
+            if (n + 1 < tiles) turn(s1, s0, n + 1, 1);
         }
     }
-
-    l = both_sum(l);
-    if (i >= p.Lq) return;
-    const float nan = __builtin_nanf("");
-    float f = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : nan);
-    if (DROP) f *= drop.scale;
-    if (i >= e.nq) f = 0.0f;
-    if (e.bad) f = nan;
-    const bool none = i >= e.nq || !(l != 0.0f);   // no key: zeros, whatever the accumulators hold
-    char* row = (char*)a.out + (((long long)b * p.Lq + i) * p.Hq + hq) * D * (long long)sizeof(T);
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d0 = 32 * d + 8 * g + 4 * h;
-            float y[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = none ? (e.bad ? nan : 0.0f) : o[d][4 * g + r] * f;
-            if (d0 < D) Elem<T>::store4(row + d0 * (int)sizeof(T), y);
-        }
-    if (h == 0) {
-        const long long n = (long long)p.B * p.Hq * p.Lq, at_row = (long long)bh * p.Lq + i;
-        a.stats[at_row] = e.bad ? nan : none ? -__builtin_inff() : m;
-        a.stats[n + at_row] = none ? 0.0f : log2_(l) - FORWARD_SHIFT<T>;
-    }
+    f.store(e, b, hq, bh);
 }
 
-template <class T, int DP, bool BIAS, bool DROP>
+template <class T, int DP, int QT, int NW, bool BIAS, bool DROP>
 int launch_forward_as(const ForwardArgs& a, hipStream_t st) {
-    auto kernel = attention_forward_kernel<T, DP, BIAS, DROP>;
-    const int lds = 2 * Tile<T, DP>::bytes(64) + (BIAS ? (2 * a.p.max_distance + 1) * 4 : 0);
+    auto kernel = attention_forward_kernel<T, DP, QT, NW, BIAS, DROP>;
+    const int lds = Forward<T, DP, QT, NW, BIAS, DROP>::LDS +
+                    (BIAS ? (2 * a.p.max_distance + 1) * 4 : 0);
     D2P_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                 lds));
-    const long long n = (long long)a.p.B * a.p.Hq * cdiv(a.p.Lq, 128);
+    const long long n = (long long)a.p.B * a.p.Hq * cdiv(a.p.Lq, 32 * QT * NW);
     D2P_REQUIRE(n <= 0x7fffffffLL, "too many query blocks");
     if (n == 0) return D2P_OK;
-    D2P_LAUNCH("attention_forward", kernel, dim3((unsigned)n), dim3(256), lds, st, a);
+    D2P_LAUNCH("attention_forward", kernel, dim3((unsigned)n), dim3(64 * NW), lds, st, a);
     D2P_HIP(hipGetLastError());
     return D2P_OK;
 }
 
+// Waves of 32 queries in a workgroup: eight share K and V tiles where features are many and
+// the card is filled twice even so ([2, 8192, 16, 128] bfloat16: 989 us, 1112 TFLOP/s, against
+// 1117 with four; [2, 4096, 16, 128] causal: 147 against 154); four otherwise, whose blocks
+// fill it sooner ([4, 4096, 16, 64]: 330 us against 357; [4, 1023, 12, 80] causal: 40 against 46).
+template <class T, int DP, bool BIAS, bool DROP>
+int launch_forward_shape(const ForwardArgs& a, hipStream_t st) {
+    if constexpr (DP == 128 && sizeof(T) == 2)
+        if ((long long)a.p.B * a.p.Hq * cdiv(a.p.Lq, 256) >= 2LL * device_cus())
+            return launch_forward_as<T, DP, 1, 8, BIAS, DROP>(a, st);
+    return launch_forward_as<T, DP, 1, 4, BIAS, DROP>(a, st);
+}
+
 template <class T, int DP> int launch_forward_dp(const ForwardArgs& a, hipStream_t st) {
     if (a.p.bias)
-        return a.p.drop ? launch_forward_as<T, DP, true, true>(a, st)
-                        : launch_forward_as<T, DP, true, false>(a, st);
-    return a.p.drop ? launch_forward_as<T, DP, false, true>(a, st)
-                    : launch_forward_as<T, DP, false, false>(a, st);
+        return a.p.drop ? launch_forward_shape<T, DP, true, true>(a, st)
+                        : launch_forward_shape<T, DP, true, false>(a, st);
+    return a.p.drop ? launch_forward_shape<T, DP, false, true>(a, st)
+                    : launch_forward_shape<T, DP, false, false>(a, st);
 }
 
 template <class T> int launch_forward(const ForwardArgs& a, hipStream_t st) {

@@ -211,6 +211,56 @@ template <class T, int DP, int R, int N> struct Stage {
     }
 };
 
+// One tile of R rows straight from memory to LDS, by the waves of a workgroup together: an
+// instruction brings 64 chunks to consecutive slots, and each lane fetches the chunk that
+// belongs in its slot.  Out of range (past the last row, past D) comes as zeros.  Inline
+// assembly, so that the compiler does not make every later LDS read wait for it: wait_dma()
+// and a barrier do, one tile later.  M0 takes the LDS address; the compiler uses M0 for
+// nothing here.
+template <class T, int DP, int R, int NW> struct TileDma {
+    using TL = Tile<T, DP>;
+    static constexpr int INSTR = R * TL::NCH / 64, COUNT = (INSTR + NW - 1) / NW;
+    static constexpr int ROWS = 64 / TL::NCH;   // of an instruction
+    unsigned off[COUNT];
+    __device__ __forceinline__ void init(const Rows& src, int wave, int lane) {
+#pragma unroll
+        for (int n = 0; n < COUNT; ++n) {
+            const int r = (wave + NW * n) * ROWS + lane / TL::NCH;
+            off[n] = src.at(r, (lane % TL::NCH) ^ TL::swz(r));
+        }
+    }
+    __device__ __forceinline__ void issue(const Rows& src, int r0, const u4v* tile,
+                                          int wave) const {
+        const long long left = ((long long)src.rows - r0 - 1) * src.stride + src.chunks * 16;
+        const unsigned n = src.rows <= r0 ? 0u : left > 0x7fffffffLL ? 0x7fffffffu : (unsigned)left;
+        const uint64_t b = (uint64_t)(src.base + (long long)r0 * src.stride);
+        const u4v r = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)b),
+                       (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(b >> 32)) & 0xffffu,
+                       (unsigned)__builtin_amdgcn_readfirstlane(n), 0x00020000u};
+        const unsigned lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)tile;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+#pragma unroll
+        for (int k = 0; k < COUNT; ++k) {
+            const int q = __builtin_amdgcn_readfirstlane(wave) + NW * k;
+            if (INSTR % NW == 0 || q < INSTR)
+                __asm__ volatile("s_mov_b32 m0, %2\n\t"
+                                 "s_nop 0\n\t"
+                                 "buffer_load_dwordx4 %0, %1, 0 offen lds"
+                                 :: "v"(off[k]), "s"(r), "s"(lds + q * 1024) : "memory", "m0");
+        }
+#pragma clang diagnostic pop
+    }
+};
+// Every direct load of this wave has arrived.
+__device__ __forceinline__ void wait_dma() { __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// A barrier that waits for nothing but the waves.
+__device__ __forceinline__ void meet() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // both halves of a wave: the larger, the sum
 __device__ __forceinline__ float both_max(float x) {
     const u2v r = bits<u2v>(__builtin_amdgcn_permlane32_swap(bits<unsigned>(x), bits<unsigned>(x),
@@ -382,6 +432,22 @@ __device__ __forceinline__ void load_bias(float* lds, const d2p_attention_params
 __device__ __forceinline__ unsigned near_xcd(unsigned w, unsigned n) {
     const unsigned x = w & 7, q = n >> 3, r = n & 7;
     return x * q + (x < r ? x : r) + (w >> 3);
+}
+
+// Head (of all heads of the batch) and block of workgroup w.  An XCD takes whole heads, so
+// that their blocks share its L2.  Blocks of equal work go head by head; where work falls
+// with the block (`falling`: causal order), an XCD goes through the heaviest blocks of all
+// its heads first, and the light ones fill the end.
+__device__ __forceinline__ void place(unsigned w, int heads, int blocks, bool falling, int* head,
+                                      int* block) {
+    const unsigned x = near_xcd(w, (unsigned)heads * blocks);
+    *head = x / blocks;
+    *block = x % blocks;
+    if (falling && heads % 8 == 0) {
+        const unsigned own = heads / 8, n = w >> 3;   // of this XCD: its heads, its n-th turn
+        *head = (w & 7) * own + n % own;
+        *block = n / own;
+    }
 }
 
 // ---------------------------------------------------------------------------
