@@ -57,13 +57,15 @@ static bool aligned(const void* x) { return ((uintptr_t)x & 15) == 0; }
 
 // Parts of the backward pass's workspace, in floats.
 struct BackwardLayout {
-    size_t delta, partial, largest;
+    size_t heads, delta, partial, largest;
     explicit BackwardLayout(const d2p_attention_params& p) {
+        // first, for its 16-byte accesses (D is a multiple of 8)
+        heads = split_groups(p) ? 2 * (size_t)p.B * p.Lk * p.Hq * p.D : 0;
         delta = (size_t)p.B * p.Hq * p.Lq;
         partial = p.bias ? (size_t)p.B * p.Hq * query_blocks(p) * (2 * p.max_distance + 1) : 0;
         largest = p.dtype == D2P_FLOAT16 ? (size_t)p.B * p.Hq * query_blocks(p) * 4 : 0;
     }
-    size_t bytes() const { return (delta + partial + largest) * 4; }
+    size_t bytes() const { return (heads + delta + partial + largest) * 4; }
 };
 
 }  // namespace enc
@@ -126,10 +128,14 @@ extern "C" int d2p_attention_backward(const d2p_attention_params* p, const void*
                     "tensors must be aligned to 16 bytes");
     }
     const BackwardLayout lay(*p);
+    D2P_REQUIRE(((uintptr_t)workspace & 15) == 0, "workspace must be aligned to 16 bytes");
     D2P_REQUIRE(lay.bytes() == 0 || (workspace && workspace_bytes >= lay.bytes()),
                 "workspace too small");
-    BackwardArgs a{*p, grad, q, k, v, out, stats, dq, dk, dv, dbias, (float*)workspace,
-                   (float*)workspace + lay.delta, (float*)workspace + lay.delta + lay.partial};
+    BackwardArgs a{*p, grad, q, k, v, out, stats, dq, dk, dv, dbias};
+    a.heads = lay.heads ? (float*)workspace : nullptr;
+    a.delta = (float*)workspace + lay.heads;
+    a.partial = a.delta + lay.delta;
+    a.largest = a.partial + lay.partial;
     if (p->B == 0 && !dbias) return D2P_OK;
     return p->dtype == D2P_FLOAT32   ? launch_backward_f32(a, st)
            : p->dtype == D2P_FLOAT16 ? launch_backward_f16(a, st)

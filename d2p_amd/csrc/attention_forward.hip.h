@@ -23,32 +23,51 @@ struct ForwardArgs {
     float* stats;
 };
 
-// The scores of one 32 x 32 tile, lane = query, accumulators = keys j0 + 8 g + 4 h + r: in
-// units of log2, with the bias, -inf where the key is at or past `limit`.  at: the query's
-// place among the keys; far: 0, or the bias of the whole tile is that of one clipped
-// distance (-1, 1: see bias_reach).
-template <bool BIAS, bool FULL>
-__device__ __forceinline__ void score_tile(f16v s, float c, const float* bias, int R, int far,
-                                           int j0, int at, int limit, int lane, float* x) {
-    const int j = j0 + 4 * (lane >> 5);
-    float b = 0.0f;
-    if (BIAS && far) b = bias[far < 0 ? 0 : 2 * R];
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-        const int n = 8 * (v >> 2) + (v & 3);
-        float y = s[v] * c;
-        if (BIAS) {
-            if (far == 0) b = bias[min(max(j + n - at, -R), R) + R];
-            y += b;
-        }
-        x[v] = FULL || j + n < limit ? y : -__builtin_inff();
-    }
-}
-
 // Whether every pair of queries placed at0 .. at0 + 31 and keys j0 .. j1 lies at or past
 // the clipping distance behind (-1) or ahead (1); 0: neither.
 __device__ __forceinline__ int bias_reach(int j0, int j1, int at0, int R) {
     return j1 - at0 <= -R ? -1 : j0 - (at0 + 31) >= R ? 1 : 0;
+}
+
+// s c + bias, in units of log2, of 16 accumulators: distance d + SIGN (8 g + r) for v = 4 g + r
+template <int SIGN>
+__device__ __forceinline__ void add_bias_at(f16v& s, float c, const float* bias, int R, int d) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        const int n = d + SIGN * (8 * (v >> 2) + (v & 3));
+        s[v] = fmaf(s[v], c, bias[min(max(n, -R), R) + R]);
+    }
+}
+// a tile whose distances are all within the table: no clipping
+template <int SIGN>
+__device__ __forceinline__ void add_bias_inside(f16v& s, float c, const float* bias, int R, int d) {
+    const float* b = bias + R + d;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) s[v] = fmaf(s[v], c, b[SIGN * (8 * (v >> 2) + (v & 3))]);
+}
+template <int SIGN>
+__device__ __forceinline__ void add_bias_to(f16v& s, float c, const float* bias, int R, int j0,
+                                            int at0, int d) {
+    const int far = bias_reach(j0, j0 + 31, at0, R);
+    if (far) {
+        const float b = bias[far < 0 ? 0 : 2 * R];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = fmaf(s[v], c, b);
+    } else if (j0 - (at0 + 31) >= -R && j0 + 31 - at0 <= R) {
+        add_bias_inside<SIGN>(s, c, bias, R, d);
+    } else {
+        add_bias_at<SIGN>(s, c, bias, R, d);
+    }
+}
+// lane = query placed at, accumulators = keys from j0; at0: the tile's first query
+__device__ __forceinline__ void add_bias(f16v& s, float c, const float* bias, int R, int j0,
+                                         int at0, int at, int lane) {
+    add_bias_to<1>(s, c, bias, R, j0, at0, j0 + 4 * (lane >> 5) - at);
+}
+// lane = key j0 + l % 32, accumulators = queries placed from at0 on
+__device__ __forceinline__ void add_bias_by_key(f16v& s, float c, const float* bias, int R,
+                                                int j0, int at0, int lane) {
+    add_bias_to<-1>(s, c, bias, R, j0, at0, j0 + (lane & 31) - at0 - 4 * (lane >> 5));
 }
 
 // Shared by the waves of a workgroup: K and V tiles of 64 keys, two of each, which go to
@@ -121,21 +140,8 @@ template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward 
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                if (BIAS) {
-                    const int j = j0 + 32 * k, far = bias_reach(j, j + 31, at0 + 32 * t, R);
-                    if (far) {
-                        const float b = bias[far < 0 ? 0 : 2 * R];
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) s[k][t][v] = fmaf(s[k][t][v], c, b);
-                    } else {
-                        const int d = j + 4 * h - at[t];
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) {
-                            const int n = d + 8 * (v >> 2) + (v & 3);
-                            s[k][t][v] = fmaf(s[k][t][v], c, bias[min(max(n, -R), R) + R]);
-                        }
-                    }
-                }
+                if (BIAS)
+                    add_bias(s[k][t], c, bias, R, j0 + 32 * k, at0 + 32 * t, at[t], lane);
                 if (!full) {
                     const int left = limit[t] - (j0 + 32 * k + 4 * h);
 #pragma unroll

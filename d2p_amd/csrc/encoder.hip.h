@@ -292,6 +292,13 @@ __device__ __forceinline__ int exponent(float x) {
     return e == 0 ? -100 : e == 255 ? 0 : e - 126;
 }
 
+// x, which the compiler must take for new: what is computed from it in a loop is computed
+// there, in place of a register (or a spill) for each address.
+__device__ __forceinline__ int fresh(int x) {
+    __asm__ volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
 
