@@ -628,8 +628,8 @@ int launch_dq_as(const BackwardArgs& a, hipStream_t st) {
     using K = Dq<T, DP, BIAS, DROP, DBIAS>;
     auto kernel = attention_dq_kernel<T, DP, BIAS, DROP, DBIAS>;
     const int lds = K::lds(a.p);
-    D2P_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                lds));
+    static LdsAllowed known;
+    D2P_TRY(allow_lds((const void*)kernel, known));
     const long long n = (long long)a.p.B * a.p.Hq * query_blocks(a.p);
     D2P_REQUIRE(n <= 0x7fffffffLL, "too many query blocks");
     if (n == 0) return D2P_OK;
@@ -650,8 +650,8 @@ int launch_dkv_as(const BackwardArgs& a, hipStream_t st) {
     using K = Dkv<T, DP>;
     auto kernel = attention_dkv_kernel<T, DP, BIAS, DROP>;
     const int lds = K::lds(a.p);
-    D2P_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                lds));
+    static LdsAllowed known;
+    D2P_TRY(allow_lds((const void*)kernel, known));
     const long long n = (long long)a.p.B * (a.heads ? a.p.Hq : a.p.Hkv) * cdiv(a.p.Lk, K::KEYS);
     D2P_REQUIRE(n <= 0x7fffffffLL, "too many key blocks");
     if (n == 0) return D2P_OK;

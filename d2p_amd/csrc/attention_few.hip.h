@@ -327,8 +327,8 @@ template <class T, int DP, bool BIAS> int launch_few_as(const FewArgs& a, hipStr
     const d2p_attention_params& p = a.f.p;
     const int lds = std::max(4 * Tile<T, DP>::bytes(32), 4 * 32 * (DP + 4) * 4) + 256 * 4 +
                     (BIAS ? (2 * p.max_distance + 1) * 4 : 0);
-    D2P_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                lds));
+    static LdsAllowed known;
+    D2P_TRY(allow_lds((const void*)kernel, known));
     const long long n = (long long)p.B * p.Hkv * a.plan.row_tiles * a.plan.parts;
     D2P_LAUNCH("attention_few", kernel, dim3((unsigned)n), dim3(256), lds, st, a);
     D2P_HIP(hipGetLastError());

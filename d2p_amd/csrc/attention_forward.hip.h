@@ -305,8 +305,8 @@ int launch_forward_as(const ForwardArgs& a, hipStream_t st) {
     auto kernel = attention_forward_kernel<T, DP, QT, NW, BIAS, DROP>;
     const int lds = Forward<T, DP, QT, NW, BIAS, DROP>::LDS +
                     (BIAS ? (2 * a.p.max_distance + 1) * 4 : 0);
-    D2P_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                lds));
+    static LdsAllowed known;
+    D2P_TRY(allow_lds((const void*)kernel, known));
     const long long n = (long long)a.p.B * a.p.Hq * cdiv(a.p.Lq, 32 * QT * NW);
     D2P_REQUIRE(n <= 0x7fffffffLL, "too many query blocks");
     if (n == 0) return D2P_OK;

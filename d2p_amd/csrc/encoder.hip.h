@@ -15,6 +15,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "capi_util.hip.h"
 #include "../../include/d2p_amd_encoder.h"
 
@@ -463,6 +465,21 @@ __device__ __forceinline__ void place(unsigned w, int heads, int blocks, bool fa
 inline int type_bytes(int dtype) { return dtype == D2P_FLOAT32 ? 4 : 2; }
 inline int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 __host__ __device__ inline int cdiv(int a, int b) { return (int)(((long long)a + b - 1) / b); }
+
+// Lets `kernel` have up to a compute unit's LDS on the current device; asked for once for
+// each kernel and device (`known`: the kernel's own, zeros at first).
+struct LdsAllowed {
+    std::atomic<bool> on[64];
+};
+inline int allow_lds(const void* kernel, LdsAllowed& known) {
+    int dev = 0;
+    D2P_HIP(hipGetDevice(&dev));
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep && known.on[dev].load(std::memory_order_relaxed)) return D2P_OK;
+    D2P_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    if (keep) known.on[dev].store(true, std::memory_order_relaxed);
+    return D2P_OK;
+}
 
 // Every argument of an attention call that the host can see.
 int check_attention(const d2p_attention_params* p);

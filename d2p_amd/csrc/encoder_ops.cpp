@@ -166,10 +166,12 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor& q_, const Tensor& k_,
     TORCH_CHECK(q_.is_cuda(), "q must be a CUDA tensor");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q_.device());
     // sizes and types are checked before anything is copied
-    attention_params(q_, k_, v_, lengths, causal, scale, bias, buckets, dropout, seed, seed_tensor);
+    auto p = attention_params(q_, k_, v_, lengths, causal, scale, bias, buckets, dropout, seed,
+                              seed_tensor);
     const Tensor q = readable(q_), k = readable(k_), v = readable(v_);
-    const auto p = attention_params(q, k, v, lengths, causal, scale, bias, buckets, dropout, seed,
-                                    seed_tensor);
+    p.q = strides_of(q);
+    p.k = strides_of(k);
+    p.v = strides_of(v);
     Tensor out = torch::empty(q.sizes(), q.options());
     Tensor stats = torch::empty({2, p.B, p.Hq, p.Lq}, q.options().dtype(torch::kFloat32));
     const size_t bytes = d2p_attention_workspace_bytes(&p);
@@ -188,7 +190,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(
     const OptTensor& seed_tensor, bool bias_grad) {
     TORCH_CHECK(q_.is_cuda(), "q must be a CUDA tensor");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q_.device());
-    attention_params(q_, k_, v_, lengths, causal, scale, bias, buckets, dropout, seed, seed_tensor);
+    auto p = attention_params(q_, k_, v_, lengths, causal, scale, bias, buckets, dropout, seed,
+                              seed_tensor);
     check_4d(grad_, q_, "grad");
     check_4d(out_, q_, "out");
     TORCH_CHECK(grad_.sizes() == q_.sizes() && out_.sizes() == q_.sizes(),
@@ -199,8 +202,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(
     TORCH_CHECK(!bias_grad || given(bias), "a bias gradient needs a bias");
     const Tensor q = readable(q_), k = readable(k_), v = readable(v_), grad = readable(grad_);
     const Tensor out = out_.contiguous();
-    auto p = attention_params(q, k, v, lengths, causal, scale, bias, buckets, dropout, seed,
-                              seed_tensor);
+    p.q = strides_of(q);
+    p.k = strides_of(k);
+    p.v = strides_of(v);
     p.grad = strides_of(grad);
     Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()),
            dv = torch::empty(v.sizes(), v.options());
@@ -227,6 +231,15 @@ auto call_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTe
     return op.call(q, k, v, lengths, causal, scale, bias, buckets, dropout, seed, seed_tensor);
 }
 
+// A backward pass that nobody differentiates skips the autograd layer of the operators it
+// calls; in one that somebody does, that layer makes their derivative raise.
+struct BelowAutograd {
+    c10::optional<at::AutoDispatchBelowADInplaceOrView> guard;
+    BelowAutograd() {
+        if (!at::GradMode::is_enabled()) guard.emplace();
+    }
+};
+
 OptTensor saved(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
 class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
@@ -251,6 +264,7 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const auto s = ctx->get_saved_variables();
         const bool bias_grad = ctx->saved_data["bias"].toBool();
+        BelowAutograd below;
         static auto op = operator_handle<decltype(attention_backward)>("d2p_amd::attention_backward");
         auto [dq, dk, dv, db] = op.call(
             grads[0], s[0], s[1], s[2], s[3], s[4], saved(s[5]), ctx->saved_data["causal"].toBool(),
@@ -411,15 +425,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rope_backward(
     in.p.gk = strides_of(gk);
     Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
     const auto f32 = q.options().dtype(torch::kFloat32);
-    Tensor dw = torch::empty({2, weight_grads ? q.size(3) : 0}, f32);
+    Tensor dwq = torch::empty({weight_grads ? q.size(3) : 0}, f32), dwk = torch::empty_like(dwq);
     const size_t bytes = weight_grads ? d2p_qk_norm_rope_backward_workspace_bytes(&in.p) : 0;
     Tensor ws = workspace(bytes, q);
-    float* w = weight_grads ? dw.data_ptr<float>() : nullptr;
     D2P_CALL(d2p_qk_norm_rope_backward(&in.p, gq.data_ptr(), gk.data_ptr(), in.q.data_ptr(),
-                                       in.k.data_ptr(), dq.data_ptr(), dk.data_ptr(), w,
-                                       w ? w + q.size(3) : nullptr, ws.data_ptr(), bytes,
-                                       current_stream()));
-    return {dq, dk, dw.select(0, 0), dw.select(0, 1)};
+                                       in.k.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                       weight_grads ? dwq.data_ptr<float>() : nullptr,
+                                       weight_grads ? dwk.data_ptr<float>() : nullptr,
+                                       ws.data_ptr(), bytes, current_stream()));
+    return {dq, dk, dwq, dwk};
 }
 
 auto call_norm(const Tensor& q, const Tensor& k, const OptTensor& q_weight,
@@ -448,6 +462,7 @@ class QkNormRopeFunction : public torch::autograd::Function<QkNormRopeFunction> 
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const auto s = ctx->get_saved_variables();
         const bool weights = ctx->saved_data["weights"].toBool();
+        BelowAutograd below;
         static auto op =
             operator_handle<decltype(qk_norm_rope_backward)>("d2p_amd::qk_norm_rope_backward");
         auto [dq, dk, dwq, dwk] = op.call(
