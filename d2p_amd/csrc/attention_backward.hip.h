@@ -19,7 +19,7 @@ struct BackwardArgs {
     const float* stats;
     void *dq, *dk, *dv, *dbias;
     float* delta;     // [B, Hq, Lq]: sum_j p_ij dp_ij = <out_i, grad_i>
-    float* partial;   // [B Hq blocks of queries, 2 R + 1]: sums of ds by clipped distance
+    float* partial;   // [Hq][B blocks of queries][2 R + 1]: sums of ds by clipped distance
     float* heads;     // [2][B, Lk, Hq, D]: dK, dV of each query head where a group is split
     float* largest;   // [B Hq blocks of queries, 4 waves]: largest |grad| (half precision)
 };
@@ -29,12 +29,11 @@ __host__ __device__ inline int query_blocks(const d2p_attention_params& p) {
 }
 
 // Sums of ds by clipped distance, for the bias's gradient.  A tile at or past the clipping
-// distance adds to one register.  Another goes to LDS, half a tile (16 queries) at a time,
-// skewed so that a diagonal is a column: lane d sums column d.  What lies between the
-// diagonals is zero from the start and never written.  Lanes and waves have their own places,
-// joined at the end in a fixed order.
+// distance adds to one register.  Another goes to LDS skewed, so that a diagonal is a column:
+// lane d sums column d.  What lies between the diagonals is zero from the start and never
+// written.  Lanes and waves have their own places, joined at the end in a fixed order.
 struct BiasSums {
-    static constexpr int PITCH = 48, TILE = 16 * PITCH;   // 47 diagonals
+    static constexpr int PITCH = 64, TILE = 32 * PITCH;   // 63 diagonals
     float behind = 0.0f, ahead = 0.0f, near = 0.0f;   // sums of ds
     float p_behind = 0.0f, p_ahead = 0.0f;            // of p
     // ds, p: lane = query, accumulators = keys from j0; at0: place of the wave's first query;
@@ -55,31 +54,24 @@ struct BiasSums {
             return;
         }
         near += s;
-        const int q = lane & 15;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int q = lane & 31;
+        float* row = tile + q * PITCH + 4 * (lane >> 5) + 31 - q;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (((lane >> 4) & 1) == half) {
-                float* row = tile + q * PITCH + 4 * (lane >> 5) + 15 - q;
+        for (int v = 0; v < 16; ++v) row[8 * (v >> 2) + (v & 3)] = SCALED ? ds[v] * down : ds[v];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        float t[4] = {};
 #pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    row[8 * (v >> 2) + (v & 3)] = SCALED ? ds[v] * down : ds[v];
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (lane >= 47) continue;
-            float t[4] = {};
-#pragma unroll
-            for (int r = 0; r < 16; ++r) t[r & 3] += tile[r * PITCH + lane];
-            const float sum = (t[0] + t[1]) + (t[2] + t[3]);
-            const int d = j0 - (at0 + 16 * half) + lane - 15;
-            // the ends of the table belong to the registers' sums; these pairs' p are not in
-            // p_behind, p_ahead, so they stay out of the correction
-            hist[min(max(d, -R), R) + R] += d > -R && d < R ? sum : 0.0f;
-            if (d <= -R) edge_lo += sum;
-            else if (d >= R) edge_hi += sum;
-        }
+        for (int r = 0; r < 32; ++r) t[r & 3] += tile[r * PITCH + lane];
+        const float sum = (t[0] + t[1]) + (t[2] + t[3]);
+        const int d = j0 - at0 + lane - 31;   // (lane 63: no diagonal, zeros)
+        // the ends of the table belong to the registers' sums; these pairs' p are not in
+        // p_behind, p_ahead, so they stay out of the correction
+        if (d > -R && d < R) hist[d + R] += sum;
+        else if (d <= -R) edge_lo += sum;
+        else edge_hi += sum;
     }
     float edge_lo = 0.0f, edge_hi = 0.0f;   // of tiles that reach past an end in part
 };
@@ -92,8 +84,9 @@ struct BiasSums {
 // reads, as many cycles as the MFMAs for four SIMDs.  Two waves a SIMD.
 template <class T, int DP, bool BIAS, bool DROP, bool DBIAS> struct Dq {
     static constexpr int NW = 4, ROWS = 32 * NW;
-    // two workgroups of a compute unit fit its LDS
-    static constexpr int BK = DBIAS && DP * sizeof(T) == 256 ? 32 : 64;
+    // two workgroups of a compute unit fit its LDS with the skewed tiles (one, with 32 bits)
+    static constexpr int BK = DBIAS && (sizeof(T) == 2 ? Tile<T, DP>::ROW == 256
+                                                       : Tile<T, DP>::ROW == 512) ? 32 : 64;
     static constexpr int TILE = Tile<T, DP>::bytes(BK) / 16;
     static int lds(const d2p_attention_params& p) {
         const int span = 2 * p.max_distance + 1;
@@ -114,7 +107,7 @@ attention_dq_kernel(BackwardArgs a) {
     float* bias = (float*)(sm + 4 * K::TILE);
     const d2p_attention_params& p = a.p;
     const int R = p.max_distance, span = 2 * R + 1;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), h = lane >> 5;
     float* tile = bias + span + wave * BiasSums::TILE;
     float* hists = bias + span + NW * BiasSums::TILE;
     const int nb = query_blocks(p);
@@ -192,7 +185,9 @@ attention_dq_kernel(BackwardArgs a) {
     const float ups = kept * up;
     f16v dq[DT] = {};
     BiasSums sums;
+    // keys that all, that any of the wave's queries see
     const int wave_full = e.limit(p, wq);
+    const int wave_end = wq < e.nq ? e.limit(p, min(wq + 32, e.nq) - 1) : 0;
     const int limit = e.limit(p, i);
 
     // probabilities x and kept gradients dp (not yet scaled) of 32 keys of a tile
@@ -229,6 +224,7 @@ attention_dq_kernel(BackwardArgs a) {
             dmk.issue(kr, (n + 1) * BK, Ks + (buf ^ 1) * K::TILE, wave);
             dmv.issue(vr, (n + 1) * BK, Vs + (buf ^ 1) * K::TILE, wave);
         }
+        if (n * BK >= wave_end) return;
         const u4v *kt = Ks + buf * K::TILE, *vt = Vs + buf * K::TILE;
         if (n == 0 && wave_full <= BK) {
             // Rows whose keys are all here: delta from p and dp themselves.  <out, grad>
@@ -290,7 +286,7 @@ attention_dq_kernel(BackwardArgs a) {
             hist[2 * R] += hi;
         }
         __syncthreads();
-        float* to = a.partial + ((long long)bh * nb + qb) * span;
+        float* to = a.partial + (((long long)hq * p.B + b) * nb + qb) * span;
         for (int t = tid; t < span; t += 64 * NW) {
             const float s = hists[t] + hists[span + t] + hists[2 * span + t] + hists[3 * span + t];
             to[t] = e.bad ? __builtin_nanf("") : s;
@@ -325,7 +321,7 @@ attention_dq_kernel(BackwardArgs a) {
 // the tiles of queries).
 template <class T, int DP> struct Dkv {
     static constexpr int NW = 4, KEYS = 32 * NW;
-    static constexpr bool WIDE = DP * sizeof(T) >= 256;   // V in LDS
+    static constexpr bool WIDE = Tile<T, DP>::ROW >= 256;   // V in LDS
     static constexpr int BQ = WIDE ? 32 : 64;
     static constexpr int TILE = Tile<T, DP>::bytes(BQ) / 16;
     static constexpr int V = WIDE ? Tile<T, DP>::bytes(KEYS) / 16 : 0;
@@ -348,7 +344,11 @@ attention_dkv_kernel(BackwardArgs a) {
     float* bias = stats + 2 * 3 * BQ;
     const d2p_attention_params& p = a.p;
     const int R = p.max_distance;
+    // (a wave's place as lanes' numbers: known to be the same in all of them, it makes branches
+    // of the masks, which the products of two tiles no longer cross: 649 -> 680 us for
+    // [4, 4096, 16, 64] bfloat16)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int mine = wave_of(tid);
     const int nb = cdiv(p.Lk, K::KEYS), group = p.Hq / p.Hkv;
     const bool split = a.heads != nullptr;   // a workgroup for each query head
     int bh, block;
@@ -373,8 +373,8 @@ attention_dkv_kernel(BackwardArgs a) {
         }
         if (K::WIDE) {
             TileDma<T, DP, K::KEYS, NW> dmv;
-            dmv.init(vr, wave, lane);
-            dmv.issue(vr, k0, Vs, wave);
+            dmv.init(vr, mine, lane);
+            dmv.issue(vr, k0, Vs, mine);
         }
     }
     auto vf = [&](int s, int ln) {
@@ -416,8 +416,8 @@ attention_dkv_kernel(BackwardArgs a) {
         }
         const float ups = kept * up;
         TileDma<T, DP, BQ, NW> dmq, dmg;
-        dmq.init(qr, wave, lane);
-        dmg.init(gr, wave, lane);
+        dmq.init(qr, mine, lane);
+        dmg.init(gr, mine, lane);
         // a row's statistics, one thread a row, on their way to LDS
         float sm_ = 0.0f, sl_ = 0.0f, sd_ = 0.0f;
         auto load_stats = [&](int i0) {
@@ -445,8 +445,8 @@ attention_dkv_kernel(BackwardArgs a) {
         __syncthreads();   // the head before is done with LDS
         load_stats(first);
         store_stats(0);
-        dmq.issue(qr, first, Qs, wave);
-        dmg.issue(gr, first, Gs, wave);
+        dmq.issue(qr, first, Qs, mine);
+        dmg.issue(gr, first, Gs, mine);
         if (BIAS) load_bias<T>(bias, p, hq, tid, 64 * NW);
 
         auto turn = [&](int n, int buf) {
@@ -455,10 +455,10 @@ attention_dkv_kernel(BackwardArgs a) {
             meet();
             if (n + 1 < tiles) {
                 load_stats(i0 + BQ);
-                dmq.issue(qr, i0 + BQ, Qs + (buf ^ 1) * K::TILE, wave);
-                dmg.issue(gr, i0 + BQ, Gs + (buf ^ 1) * K::TILE, wave);
+                dmq.issue(qr, i0 + BQ, Qs + (buf ^ 1) * K::TILE, mine);
+                dmg.issue(gr, i0 + BQ, Gs + (buf ^ 1) * K::TILE, mine);
             }
-            const int ln = K::WIDE ? fresh(lane) : lane;
+            const int ln = K::WIDE ? fresh(lane, n) : lane;
             const u4v *qt = Qs + buf * K::TILE, *gt = Gs + buf * K::TILE;
             const float* st = stats + buf * 3 * BQ;
 #pragma unroll
@@ -498,7 +498,7 @@ attention_dkv_kernel(BackwardArgs a) {
                 }
 #pragma unroll
                 for (int f = 0; f < TL::FRAGS; ++f) {
-                    const u4v pf = Elem<T>::pack(pr + TL::PER * f);
+                    u4v pf = Elem<T>::pack(pr + TL::PER * f);
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
                         dv[d] = Elem<T>::mma(TL::frag_t(gt, 32 * t, 32 * d, f, ln), pf, dv[d]);
@@ -589,19 +589,22 @@ __global__ void __launch_bounds__(1024) bias_grad_kernel(BackwardArgs a, int blo
     for (int t = tid; t < span; t += 1024) map[t] = p.buckets[t];
     for (int c0 = 0; c0 < chunks; c0 += width) {
         const int t = (c0 + wave % width) * 64 + lane, slice = wave / width;
-        float s[4] = {};
+        float s[16] = {};
         if (t < span && slice < slices) {
-            auto at = [&](int n) {
-                return a.partial[(((long long)(n / blocks) * p.Hq + h) * blocks + n % blocks) * span + t];
-            };
+            const float* from = a.partial + (long long)h * rows * span + t;
+            auto at = [&](int n) { return from[(long long)n * span]; };
             int n = slice;
-            for (; n + 3 * slices < rows; n += 4 * slices) {
+            for (; n + 15 * slices < rows; n += 16 * slices) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) s[u] += at(n + u * slices);
+                for (int u = 0; u < 16; ++u) s[u] += at(n + u * slices);
             }
             for (; n < rows; n += slices) s[0] += at(n);
         }
-        part[wave * 64 + lane] = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+        for (int u = 8; u > 0; u >>= 1)
+#pragma unroll
+            for (int r = 0; r < u; ++r) s[r] += s[r + u];
+        part[wave * 64 + lane] = s[0];
         __syncthreads();
         if (wave < width && t < span) {
             float y = 0.0f;
@@ -691,9 +694,11 @@ template <class T, int DP> int launch_backward_dp(const BackwardArgs& a, hipStre
 }
 
 template <class T> int launch_backward(const BackwardArgs& a, hipStream_t st) {
-    switch (padded(a.p.D)) {
+    switch (padded(a.p.D, a.p.dtype)) {
         case 32: D2P_TRY(launch_backward_dp<T, 32>(a, st)); break;
         case 64: D2P_TRY(launch_backward_dp<T, 64>(a, st)); break;
+        case 96:
+            if constexpr (sizeof(T) == 2) { D2P_TRY(launch_backward_dp<T, 96>(a, st)); break; }
         default: D2P_TRY(launch_backward_dp<T, 128>(a, st));
     }
     if (!a.dbias) return D2P_OK;

@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(FewArgs fa) {
     const ForwardArgs& a = fa.f;
     const d2p_attention_params& p = a.p;
     const FewPlan& pl = fa.plan;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid), h = lane >> 5;
     const int R = p.max_distance, group = p.Hq / p.Hkv, D = p.D;
     u4v* Vs = sm + wave * (TL::bytes(32) / 16);
     float* all_o = (float*)sm;                                   // [4][32][DP + 4], after the loop
@@ -282,6 +282,10 @@ __global__ void __launch_bounds__(256) attention_join_kernel(FewArgs fa) {
     }
 }
 
+inline int few_features(const d2p_attention_params& p) {
+    return p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128;
+}
+
 // Whether a call goes this way, and how it is cut.
 //
 // Both ways' times in us, from what they measured on 256 compute units.  attention_forward
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(FewArgs fa) {
 // 256 queries 267 / 38; 32 heads of 8 over 1024 keys, 128 queries: 23 / 28.
 inline bool plan_few(const d2p_attention_params& p, FewPlan* pl) {
     if (p.drop || p.B == 0 || p.Lq == 0) return false;
-    const int cus = device_cus() > 0 ? device_cus() : 256, dp = padded(p.D);
+    const int cus = device_cus() > 0 ? device_cus() : 256, dp = few_features(p);
     const bool wide = p.dtype == D2P_FLOAT32;
     const long long rows = (long long)p.Hq / p.Hkv * p.Lq;
     if (rows > 1 << 20) return false;
@@ -341,7 +345,7 @@ template <class T, int DP, bool BIAS> int launch_few_as(const FewArgs& a, hipStr
 
 template <class T> int launch_few(const FewArgs& a, hipStream_t st) {
     const bool bias = a.f.p.bias != nullptr;
-    switch (padded(a.f.p.D)) {
+    switch (few_features(a.f.p)) {
         case 32: return bias ? launch_few_as<T, 32, true>(a, st) : launch_few_as<T, 32, false>(a, st);
         case 64: return bias ? launch_few_as<T, 64, true>(a, st) : launch_few_as<T, 64, false>(a, st);
         default: return bias ? launch_few_as<T, 128, true>(a, st) : launch_few_as<T, 128, false>(a, st);

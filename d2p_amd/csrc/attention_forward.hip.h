@@ -118,14 +118,14 @@ template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward 
         }
     }
 
-    __device__ __forceinline__ void scores(f16v (&s)[2][QT], int buf) const {
+    __device__ __forceinline__ void scores(f16v (&s)[2][QT], int buf, int ln) const {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
             for (int t = 0; t < QT; ++t) s[k][t] = f16v{};
 #pragma unroll
             for (int n = 0; n < TL::STEPS; ++n) {
-                const u4v kf = TL::frag(Ks + buf * TILE, 32 * k, n, lane);
+                const u4v kf = TL::frag(Ks + buf * TILE, 32 * k, n, ln);
 #pragma unroll
                 for (int t = 0; t < QT; ++t) s[k][t] = E::mma(kf, qf[t][n], s[k][t]);
             }
@@ -184,23 +184,27 @@ template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward 
                 x[v] = exp2_(BIAS ? s[k][t][v] - ref[t] : fmaf(s[k][t][v], c, -ref[t]));
                 l[t] += x[v];
             }
-            if (DROP) {
-                const u4v kw = drop.by_query(wq + 32 * t, j0 + 32 * k, lane);
+            u4v kw;
+            if (DROP) kw = drop.by_query(wq + 32 * t, j0 + 32 * k, lane);
+            if (DROP && sizeof(T) == 4) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v) x[v] = drop.keeps(kw, v) ? x[v] : 0.0f;
             }
             // P in the type of V: its rounding is that of one factor of each product
 #pragma unroll
-            for (int f = 0; f < TL::FRAGS; ++f) pf[t][f] = E::pack(x + TL::PER * f);
+            for (int f = 0; f < TL::FRAGS; ++f) {
+                pf[t][f] = E::pack(x + TL::PER * f);
+                if (DROP && sizeof(T) == 2) pf[t][f] = drop.keep16(pf[t][f], kw, f);
+            }
         }
     }
 
-    __device__ __forceinline__ void values(const u4v (&pf)[QT][TL::FRAGS], int k, int buf) {
+    __device__ __forceinline__ void values(const u4v (&pf)[QT][TL::FRAGS], int k, int buf, int ln) {
 #pragma unroll
         for (int f = 0; f < TL::FRAGS; ++f)
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const u4v vf = TL::frag_t(Vs + buf * TILE, 32 * k, 32 * d, f, lane);
+                const u4v vf = TL::frag_t(Vs + buf * TILE, 32 * k, 32 * d, f, ln);
 #pragma unroll
                 for (int t = 0; t < QT; ++t) o[t][d] = E::mma(vf, pf[t][f], o[t][d]);
             }
@@ -250,7 +254,7 @@ attention_forward_kernel(ForwardArgs a) {
     u4v* Vs = sm + 2 * F::TILE;
     float* bias = (float*)(sm + 4 * F::TILE);
     const d2p_attention_params& p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_of(tid);
     const int nb = (p.Lq + ROWS - 1) / ROWS;
     int bh, block;
     place(blockIdx.x, p.B * p.Hq, nb, p.causal, &bh, &block);
@@ -270,14 +274,16 @@ attention_forward_kernel(ForwardArgs a) {
     if (tiles > 0) dk.issue(kr, 0, Ks, wave);
     if (BIAS) load_bias<T>(bias, p, hq, tid, 64 * NW);
     F f(a, e, qr, sm, bias, bh, q0 + 32 * QT * wave, lane);
-    const int wave_full = e.limit(p, f.wq);   // keys that all of the wave's queries see
+    // keys that all, that any of the wave's queries see
+    const int wave_full = e.limit(p, f.wq);
+    const int wave_end = f.wq < e.nq ? e.limit(p, min(f.wq + 32 * QT, e.nq) - 1) : 0;
     if (tiles > 0) {
         f16v s0[2][QT], s1[2][QT];
         wait_dma();
         __syncthreads();
         dv.issue(vr, 0, Vs, wave);
         if (tiles > 1) dk.issue(kr, BK, Ks + F::TILE, wave);
-        f.scores(s0, 0);
+        f.scores(s0, 0, lane);
         f.settle(s0, 0, BK <= wave_full);
         auto turn = [&](f16v (&now)[2][QT], f16v (&next)[2][QT], int n, int buf) {
             wait_dma();
@@ -285,12 +291,17 @@ attention_forward_kernel(ForwardArgs a) {
             if (n + 1 < tiles) dv.issue(vr, (n + 1) * BK, Vs + (buf ^ 1) * F::TILE, wave);
             if (n + 2 < tiles) dk.issue(kr, (n + 2) * BK, Ks + buf * F::TILE, wave);
             u4v p0[QT][TL::FRAGS], p1[QT][TL::FRAGS];
-            f.scores(next, buf ^ 1);   // past the last tile: of no use, and harmless
+            if (n * BK >= wave_end) return;
+            // (float32 by 128: [4, 1024, 8, 128] 207 -> 169 us; 16 bits by 128 have the registers,
+            // and lose by it: [2, 8192, 16, 128] 1045 -> 1240 us)
+            const int ln = DP * sizeof(T) == 512 ? fresh(lane, n) : lane;
+            f.scores(next, buf ^ 1, ln);   // past the wave's last tile: of no use, and harmless
             f.weights(now, 0, n * BK, p0);
-            f.values(p0, 0, buf);
+            f.values(p0, 0, buf, ln);
             f.weights(now, 1, n * BK, p1);
-            f.values(p1, 1, buf);
-            if (n + 1 < tiles) f.settle(next, (n + 1) * BK, (n + 2) * BK <= wave_full);
+            f.values(p1, 1, buf, ln);
+            if ((n + 1) * BK < wave_end)
+                f.settle(next, (n + 1) * BK, (n + 2) * BK <= wave_full);
         };
         for (int n = 0; n < tiles; n += 2) {
             turn(s0, s1, n, 0);
@@ -336,9 +347,11 @@ template <class T, int DP> int launch_forward_dp(const ForwardArgs& a, hipStream
 }
 
 template <class T> int launch_forward(const ForwardArgs& a, hipStream_t st) {
-    switch (padded(a.p.D)) {
+    switch (padded(a.p.D, a.p.dtype)) {
         case 32: return launch_forward_dp<T, 32>(a, st);
         case 64: return launch_forward_dp<T, 64>(a, st);
+        case 96:
+            if constexpr (sizeof(T) == 2) return launch_forward_dp<T, 96>(a, st);
         default: return launch_forward_dp<T, 128>(a, st);
     }
 }

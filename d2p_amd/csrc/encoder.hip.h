@@ -121,10 +121,12 @@ template <> struct Elem<__bf16> : Elem16<__bf16, b8v, b4v> {
 // A tile of rows of DP features lies in LDS row by row, chunk c of row r at slot
 // c ^ swz(r) of the row.  Sixteen rows' equal chunks (an operand's rows) and four rows'
 // four neighbouring chunks (a transposed operand's) then each cover the 64 banks once.
+// (96 features lie in rows of 128.)
 template <class T, int DP> struct Tile {
     static constexpr int PER = Elem<T>::PER;
-    static constexpr int NCH = DP / PER;          // chunks of a row
-    static constexpr int STEPS = NCH / 2;         // MFMA steps over the features
+    static constexpr int NCH = (DP == 96 ? 128 : DP) / PER;   // chunks of a row
+    static constexpr int ROW = NCH * 16;          // bytes of a row
+    static constexpr int STEPS = DP / PER / 2;    // MFMA steps over the features
     static constexpr int FRAGS = 32 / (2 * PER);  // MFMA steps over 32 rows
     static constexpr int bytes(int rows) { return rows * NCH * 16; }
 
@@ -244,7 +246,7 @@ template <class T, int DP, int R, int NW> struct TileDma {
 #pragma clang diagnostic ignored "-Winline-asm"
 #pragma unroll
         for (int k = 0; k < COUNT; ++k) {
-            const int q = __builtin_amdgcn_readfirstlane(wave) + NW * k;
+            const int q = wave + NW * k;
             if (INSTR % NW == 0 || q < INSTR)
                 __asm__ volatile("s_mov_b32 m0, %2\n\t"
                                  "s_nop 0\n\t"
@@ -294,10 +296,13 @@ __device__ __forceinline__ int exponent(float x) {
     return e == 0 ? -100 : e == 255 ? 0 : e - 126;
 }
 
-// x, which the compiler must take for new: what is computed from it in a loop is computed
-// there, in place of a register (or a spill) for each address.
-__device__ __forceinline__ int fresh(int x) {
-    __asm__ volatile("" : "+v"(x));
+// The wave of a thread, which the compiler must take for the same in all its lanes.
+__device__ __forceinline__ int wave_of(int tid) { return __builtin_amdgcn_readfirstlane(tid >> 6); }
+
+// x, which the compiler must take for new in turn n of a loop: what is computed from it is
+// computed there, in place of a register (or a spill) for each address.
+__device__ __forceinline__ int fresh(int x, int n) {
+    __asm__("" : "+v"(x) : "s"(n));
     return x;
 }
 
@@ -379,6 +384,24 @@ struct Drop {
     }
     __device__ __forceinline__ bool keeps(u4v w, int v) const {
         return ((w[v >> 2] >> (8 * (v & 3))) & 255u) >= least;
+    }
+    // Zeros for what is dropped of accumulators 8 f .. 8 f + 7 packed to 16 bits.  All four
+    // bytes of a word at once: with t's low seven bits taken off each byte under a borrow-proof
+    // top bit, u, a byte is kept if its own top bit and u's agree with t's top bit to that end
+    // (their majority with it); a byte permute spreads those bits over the packed halves.
+    __device__ __forceinline__ u4v keep16(u4v packed, u4v w, int f) const {
+        const unsigned top = 0x80808080u, low = (least & 127u) * 0x01010101u;
+        const unsigned less = least & 128u ? 0u : ~0u;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const unsigned x = w[2 * f + n], u = (x | top) - low;
+            const unsigned k = (x & u) | ((x | u) & less);
+            // selectors 8 and 9: copies of the top bits of bytes 1 and 3; 10 and 11: of
+            // bytes 0 and 2, moved up
+            packed[2 * n] &= __builtin_amdgcn_perm(k << 8, k, 0x08080a0au);
+            packed[2 * n + 1] &= __builtin_amdgcn_perm(k << 8, k, 0x09090b0bu);
+        }
+        return packed;
     }
 };
 
@@ -463,7 +486,11 @@ __device__ __forceinline__ void place(unsigned w, int heads, int blocks, bool fa
 // host side
 // ---------------------------------------------------------------------------
 inline int type_bytes(int dtype) { return dtype == D2P_FLOAT32 ? 4 : 2; }
-inline int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+// Features that the kernels for D work with; 96 with 16 bits only, where it leaves registers
+// ([4, 1023, 12 over 3, 80] half with dropout, forward and backward kernels: 168 -> 150 us).
+inline int padded(int D, int dtype) {
+    return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 && type_bytes(dtype) == 2 ? 96 : 128;
+}
 __host__ __device__ inline int cdiv(int a, int b) { return (int)(((long long)a + b - 1) / b); }
 
 // Lets `kernel` have up to a compute unit's LDS on the current device; asked for once for

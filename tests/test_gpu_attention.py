@@ -79,7 +79,8 @@ def test_sizes_and_types(cuda, size, dtype):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("size,buckets,R", [((2, 70, 70, 2, 2, 64), 16, 32), ((1, 300, 300, 2, 1, 32), 32, 128),
                                             ((1, 130, 200, 2, 2, 128), 9, 5), ((2, 40, 50, 2, 2, 8), 3, 0),
-                                            ((1, 150, 150, 1, 1, 64), 300, 1024)], ids=str)
+                                            ((1, 150, 150, 1, 1, 64), 300, 1024), ((1, 70, 130, 2, 1, 128), 5, 1024),
+                                             ((2, 90, 90, 2, 1, 96), 12, 40)], ids=str)
 def test_bias_and_its_gradient(cuda, size, buckets, R, dtype):
     for causal, bias_type in ((False, dtype), (True, F32)):
         both(inputs(3, *size, dtype, cuda, buckets, R, bias_type), causal=causal)
