@@ -190,15 +190,16 @@ attention_dq_kernel(BackwardArgs a) {
     const int wave_end = wq < e.nq ? e.limit(p, min(wq + 32, e.nq) - 1) : 0;
     const int limit = e.limit(p, i);
 
+    const int ra = TL::row_at(lane), ca = TL::col_at(lane);
     // probabilities x and kept gradients dp (not yet scaled) of 32 keys of a tile
     auto tile_of = [&](const u4v* kt, const u4v* vt, int t, int jt, float* x, f16v& dp) {
         f16v s = {};
         dp = f16v{};
 #pragma unroll
-        for (int n = 0; n < TL::STEPS; ++n) s = Elem<T>::mma(TL::frag(kt, 32 * t, n, lane), qf[n], s);
+        for (int n = 0; n < TL::STEPS; ++n) s = Elem<T>::mma(TL::frag(kt, 32 * t, n, ra), qf[n], s);
 #pragma unroll
         for (int n = 0; n < TL::STEPS; ++n)
-            dp = Elem<T>::mma(TL::frag(vt, 32 * t, n, lane), gf[n], dp);
+            dp = Elem<T>::mma(TL::frag(vt, 32 * t, n, ra), gf[n], dp);
         if (BIAS) add_bias(s, c, bias, R, jt, wq + e.off, at, lane);
         if (jt + 32 > wave_full) {
             const int left = limit - (jt + 4 * h);
@@ -259,7 +260,7 @@ attention_dq_kernel(BackwardArgs a) {
                 const u4v df = Elem<T>::pack(y + TL::PER * f);
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
-                    dq[d] = Elem<T>::mma(TL::frag_t(kt, 32 * t, 32 * d, f, lane), df, dq[d]);
+                    dq[d] = Elem<T>::mma(TL::frag_t(kt, 32 * t, 32 * d, f, ca), df, dq[d]);
             }
         }
     };
@@ -377,8 +378,9 @@ attention_dkv_kernel(BackwardArgs a) {
             dmv.issue(vr, k0, Vs, mine);
         }
     }
-    auto vf = [&](int s, int ln) {
-        return K::WIDE ? TL::frag(Vs, 32 * wave, s, ln) : vreg[s];
+    const int ra = TL::row_at(lane), ca = TL::col_at(lane);
+    auto vf = [&](int s, int rn) {
+        return K::WIDE ? TL::frag(Vs, 32 * mine, s, rn) : vreg[s];
     };
     const float c = p.scale * LOG2E;
     f16v dk[DT] = {}, dv[DT] = {};
@@ -458,7 +460,7 @@ attention_dkv_kernel(BackwardArgs a) {
                 dmq.issue(qr, i0 + BQ, Qs + (buf ^ 1) * K::TILE, mine);
                 dmg.issue(gr, i0 + BQ, Gs + (buf ^ 1) * K::TILE, mine);
             }
-            const int ln = K::WIDE ? fresh(lane, n) : lane;
+            const int rn = K::WIDE ? fresh(ra, n) : ra, cn = K::WIDE ? fresh(ca, n) : ca;
             const u4v *qt = Qs + buf * K::TILE, *gt = Gs + buf * K::TILE;
             const float* st = stats + buf * 3 * BQ;
 #pragma unroll
@@ -467,18 +469,18 @@ attention_dkv_kernel(BackwardArgs a) {
                 f16v s = {}, dp = {};
 #pragma unroll
                 for (int n = 0; n < TL::STEPS; ++n)
-                    s = Elem<T>::mma(TL::frag(qt, 32 * t, n, ln), kf[n], s);
+                    s = Elem<T>::mma(TL::frag(qt, 32 * t, n, rn), kf[n], s);
 #pragma unroll
                 for (int n = 0; n < TL::STEPS; ++n)
-                    dp = Elem<T>::mma(TL::frag(gt, 32 * t, n, ln), vf(n, ln), dp);
+                    dp = Elem<T>::mma(TL::frag(gt, 32 * t, n, rn), vf(n, rn), dp);
                 float pr[16], ds[16];
-                if (BIAS) add_bias_by_key(s, c, bias, R, wk, it + e.off, ln);
-                // every key of the wave seen by every query of the tile?
-                if (!(wk + 32 <= e.nk && (!p.causal || wk + 31 <= it + e.off))) {
-                    const int from = p.causal ? j - (it + 4 * h + e.off) : -1;
+                if (BIAS) add_bias_by_key(s, c, bias, R, wk, it + e.off, lane);
+                // (a key past the last spoils only its own row, which is not written)
+                if (p.causal && wk + 31 > it + e.off) {
+                    const int from = j - (it + 4 * h + e.off);
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
-                        s[v] = j < e.nk && 8 * (v >> 2) + (v & 3) >= from ? s[v] : -__builtin_inff();
+                        s[v] = 8 * (v >> 2) + (v & 3) >= from ? s[v] : -__builtin_inff();
                 }
                 const u4v kw = DROP ? drop.by_key(it, wk, lane) : u4v{};
 #pragma unroll
@@ -501,14 +503,14 @@ attention_dkv_kernel(BackwardArgs a) {
                     u4v pf = Elem<T>::pack(pr + TL::PER * f);
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
-                        dv[d] = Elem<T>::mma(TL::frag_t(gt, 32 * t, 32 * d, f, ln), pf, dv[d]);
+                        dv[d] = Elem<T>::mma(TL::frag_t(gt, 32 * t, 32 * d, f, cn), pf, dv[d]);
                 }
 #pragma unroll
                 for (int f = 0; f < TL::FRAGS; ++f) {
                     const u4v df = Elem<T>::pack(ds + TL::PER * f);
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
-                        dk[d] = Elem<T>::mma(TL::frag_t(qt, 32 * t, 32 * d, f, ln), df, dk[d]);
+                        dk[d] = Elem<T>::mma(TL::frag_t(qt, 32 * t, 32 * d, f, cn), df, dk[d]);
                 }
             }
             if (n + 1 < tiles) store_stats(buf ^ 1);

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(FewArgs fa) {
     f16v o[DT] = {};
     float m = -__builtin_inff(), l = 0.0f;
 
+    const int ca = TL::col_at(lane);
     u4v kf[TL::STEPS], vf[VC];
     auto load = [&](int j0) {
         const __amdgpu_buffer_rsrc_t rk = kr.from(j0), rv = vr.from(j0);
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(256) attention_few_kernel(FewArgs fa) {
             const u4v pf = Elem<T>::pack(x + TL::PER * f);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
-                o[d] = Elem<T>::mma(TL::frag_t(Vs, 0, 32 * d, f, lane), pf, o[d]);
+                o[d] = Elem<T>::mma(TL::frag_t(Vs, 0, 32 * d, f, ca), pf, o[d]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();

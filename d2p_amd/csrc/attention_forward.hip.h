@@ -118,14 +118,14 @@ template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward 
         }
     }
 
-    __device__ __forceinline__ void scores(f16v (&s)[2][QT], int buf, int ln) const {
+    __device__ __forceinline__ void scores(f16v (&s)[2][QT], int buf, int ra) const {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
 #pragma unroll
             for (int t = 0; t < QT; ++t) s[k][t] = f16v{};
 #pragma unroll
             for (int n = 0; n < TL::STEPS; ++n) {
-                const u4v kf = TL::frag(Ks + buf * TILE, 32 * k, n, ln);
+                const u4v kf = TL::frag(Ks + buf * TILE, 32 * k, n, ra);
 #pragma unroll
                 for (int t = 0; t < QT; ++t) s[k][t] = E::mma(kf, qf[t][n], s[k][t]);
             }
@@ -199,12 +199,12 @@ template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward 
         }
     }
 
-    __device__ __forceinline__ void values(const u4v (&pf)[QT][TL::FRAGS], int k, int buf, int ln) {
+    __device__ __forceinline__ void values(const u4v (&pf)[QT][TL::FRAGS], int k, int buf, int ca) {
 #pragma unroll
         for (int f = 0; f < TL::FRAGS; ++f)
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const u4v vf = TL::frag_t(Vs + buf * TILE, 32 * k, 32 * d, f, ln);
+                const u4v vf = TL::frag_t(Vs + buf * TILE, 32 * k, 32 * d, f, ca);
 #pragma unroll
                 for (int t = 0; t < QT; ++t) o[t][d] = E::mma(vf, pf[t][f], o[t][d]);
             }
@@ -268,6 +268,7 @@ attention_forward_kernel(ForwardArgs a) {
     const int end = q0 < e.nq ? e.limit(p, min(q0 + ROWS, e.nq) - 1) : 0;
     const int tiles = (end + BK - 1) / BK;
 
+    const int ra = TL::row_at(lane), ca = TL::col_at(lane);
     TileDma<T, DP, BK, NW> dk, dv;
     dk.init(kr, wave, lane);
     dv.init(vr, wave, lane);
@@ -283,7 +284,7 @@ attention_forward_kernel(ForwardArgs a) {
         __syncthreads();
         dv.issue(vr, 0, Vs, wave);
         if (tiles > 1) dk.issue(kr, BK, Ks + F::TILE, wave);
-        f.scores(s0, 0, lane);
+        f.scores(s0, 0, ra);
         f.settle(s0, 0, BK <= wave_full);
         auto turn = [&](f16v (&now)[2][QT], f16v (&next)[2][QT], int n, int buf) {
             wait_dma();
@@ -294,12 +295,13 @@ attention_forward_kernel(ForwardArgs a) {
             if (n * BK >= wave_end) return;
             // (float32 by 128: [4, 1024, 8, 128] 207 -> 169 us; 16 bits by 128 have the registers,
             // and lose by it: [2, 8192, 16, 128] 1045 -> 1240 us)
-            const int ln = DP * sizeof(T) == 512 ? fresh(lane, n) : lane;
-            f.scores(next, buf ^ 1, ln);   // past the wave's last tile: of no use, and harmless
+            constexpr bool WIDE = TL::ROW == 512;
+            const int rn = WIDE ? fresh(ra, n) : ra, cn = WIDE ? fresh(ca, n) : ca;
+            f.scores(next, buf ^ 1, rn);   // past the wave's last tile: of no use, and harmless
             f.weights(now, 0, n * BK, p0);
-            f.values(p0, 0, buf, ln);
+            f.values(p0, 0, buf, cn);
             f.weights(now, 1, n * BK, p1);
-            f.values(p1, 1, buf, ln);
+            f.values(p1, 1, buf, cn);
             if ((n + 1) * BK < wave_end)
                 f.settle(next, (n + 1) * BK, (n + 2) * BK <= wave_full);
         };

@@ -138,35 +138,45 @@ template <class T, int DP> struct Tile {
     static __device__ __forceinline__ int slot(int row, int c) {
         return row * NCH + (c ^ swz(row));
     }
-    // rows row0 .. row0 + 31 as an operand's rows, step s over the features
-    static __device__ __forceinline__ u4v frag(const u4v* tile, int row0, int s, int lane) {
-        return tile[slot(row0 + (lane & 31), 2 * s + (lane >> 5))];
+    // Fragments.  A lane's place in a tile is one number of bytes, row_at or col_at; the rest of
+    // an address is constants: chunks and the swizzle's share of a row number are combined
+    // with it by exclusive or (they touch only the bits of the chunk), the row by an offset.
+    static __device__ __forceinline__ int row_at(int lane) {
+        return 16 * slot(lane & 31, lane >> 5);
+    }
+    // rows row0 .. row0 + 31 (row0 a multiple of 32) as an operand's rows, step s over the
+    // features
+    static __device__ __forceinline__ u4v frag(const u4v* tile, int row0, int s, int ra) {
+        return *(const u4v*)((const char*)tile + row0 * ROW + (ra ^ (32 * s)));
+    }
+    static __device__ __forceinline__ int col_at(int lane) {
+        const int h = lane >> 5;
+        if (PER == 4)
+            return 16 * slot(4 * h, (lane & 31) >> 2) + 4 * (lane & 3);
+        return 16 * slot(4 * h + ((lane >> 2) & 3), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) +
+               8 * (lane & 1);
     }
     // features d0 .. d0 + 31 as an operand's rows, step f over rows row0 .. row0 + 31 in
     // the order of the accumulators: half wave h takes rows 8 g + 4 h + 0 .. 3 of
     // f = g (32 bits) or g = 2 f, 2 f + 1 (16 bits: ds_read_b64_tr_b16 gives each of 16
     // lanes one column of four rows)
     static __device__ __forceinline__ u4v frag_t(const u4v* tile, int row0, int d0, int f,
-                                                 int lane) {
-        const int h = lane >> 5;
+                                                 int ca) {
+        const char* t = (const char*)tile + row0 * ROW;
         if constexpr (PER == 4) {
-            const int d = d0 + (lane & 31);
             u4v x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = row0 + 8 * f + 4 * h + r;
-                x[r] = ((const unsigned*)tile)[4 * slot(row, d >> 2) + (d & 3)];
-            }
+            for (int r = 0; r < 4; ++r)
+                x[r] = *(const unsigned*)(t + (8 * f + r) * ROW +
+                                          (ca ^ (4 * d0) ^ (16 * swz(8 * f + r))));
             return x;
         } else {
-            const int col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
             s4v x[2];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const int row = row0 + 16 * f + 8 * n + 4 * h + ((lane >> 2) & 3);
-                const short* p = (const short*)tile + 8 * slot(row, col >> 3) + (col & 7);
+                const char* q = t + (16 * f + 8 * n) * ROW + (ca ^ (2 * d0) ^ (16 * swz(8 * n)));
                 x[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s4v*)p);
+                    (__attribute__((address_space(3))) s4v*)q);
             }
             const u2v a = bits<u2v>(x[0]), b = bits<u2v>(x[1]);
             return u4v{a.x, a.y, b.x, b.y};
@@ -220,7 +230,9 @@ template <class T, int DP, int R, int N> struct Stage {
 // belongs in its slot.  Out of range (past the last row, past D) comes as zeros.  Inline
 // assembly, so that the compiler does not make every later LDS read wait for it: wait_dma()
 // and a barrier do, one tile later.  M0 takes the LDS address; the compiler uses M0 for
-// nothing here.
+// nothing here.  (Five wait states lie between a vector instruction that writes a scalar
+// register and a load that takes its resource from there; the compiler does not look into
+// the assembly to place them.)
 template <class T, int DP, int R, int NW> struct TileDma {
     using TL = Tile<T, DP>;
     static constexpr int INSTR = R * TL::NCH / 64, COUNT = (INSTR + NW - 1) / NW;
@@ -249,7 +261,7 @@ template <class T, int DP, int R, int NW> struct TileDma {
             const int q = wave + NW * k;
             if (INSTR % NW == 0 || q < INSTR)
                 __asm__ volatile("s_mov_b32 m0, %2\n\t"
-                                 "s_nop 0\n\t"
+                                 "s_nop 4\n\t"
                                  "buffer_load_dwordx4 %0, %1, 0 offen lds"
                                  :: "v"(off[k]), "s"(r), "s"(lds + q * 1024) : "memory", "m0");
         }
