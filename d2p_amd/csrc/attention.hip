@@ -7,8 +7,7 @@
 namespace d2p_amd {
 namespace enc {
 
-int check_strides(const d2p_strides& s, int rows, int heads, int D, int dtype,
-                  const char* name) {
+int check_strides(const d2p_strides& s, int rows, int D, int dtype, const char* name) {
     const int per = dtype == D2P_FLOAT32 ? 4 : 8;   // elements of 16 bytes
     if (s.batch % per || s.row % per || s.head % per) {
         set_last_error("%s: strides must be multiples of 16 bytes", name);
@@ -22,7 +21,6 @@ int check_strides(const d2p_strides& s, int rows, int heads, int D, int dtype,
         set_last_error("%s: 128 rows must span less than 2 GiB", name);
         return D2P_ERR_ARG;
     }
-    (void)heads;
     return D2P_OK;
 }
 
@@ -47,9 +45,9 @@ int check_attention(const d2p_attention_params* p) {
         D2P_REQUIRE(p->max_distance >= 0 && p->max_distance <= 1024,
                     "max_distance must be between 0 and 1024");
     }
-    D2P_TRY(check_strides(p->q, p->Lq, p->Hq, p->D, p->dtype, "q"));
-    D2P_TRY(check_strides(p->k, p->Lk, p->Hkv, p->D, p->dtype, "k"));
-    D2P_TRY(check_strides(p->v, p->Lk, p->Hkv, p->D, p->dtype, "v"));
+    D2P_TRY(check_strides(p->q, p->Lq, p->D, p->dtype, "q"));
+    D2P_TRY(check_strides(p->k, p->Lk, p->D, p->dtype, "k"));
+    D2P_TRY(check_strides(p->v, p->Lk, p->D, p->dtype, "v"));
     return D2P_OK;
 }
 
@@ -117,7 +115,7 @@ extern "C" int d2p_attention_backward(const d2p_attention_params* p, const void*
                                       void* dv, void* dbias, void* workspace,
                                       size_t workspace_bytes, void* stream) {
     D2P_TRY(check_attention(p));
-    D2P_TRY(check_strides(p->grad, p->Lq, p->Hq, p->D, p->dtype, "grad"));
+    D2P_TRY(check_strides(p->grad, p->Lq, p->D, p->dtype, "grad"));
     D2P_REQUIRE(!dbias || p->bias, "a bias gradient needs a bias");
     hipStream_t st = (hipStream_t)stream;
     if (p->B > 0) {

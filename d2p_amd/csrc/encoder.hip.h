@@ -205,26 +205,6 @@ struct Rows {
     }
 };
 
-// One tile of R rows on its way from memory through the registers of N threads to LDS.
-template <class T, int DP, int R, int N> struct Stage {
-    using TL = Tile<T, DP>;
-    static constexpr int COUNT = R * TL::NCH / N;
-    static_assert(COUNT * N == R * TL::NCH && N % TL::NCH == 0, "a tile is whole passes");
-    u4v v[COUNT];
-    __device__ __forceinline__ void load(const Rows& src, int r0, int tid) {
-        const __amdgpu_buffer_rsrc_t b = src.from(r0);
-        const int c = tid % TL::NCH, r = tid / TL::NCH;
-#pragma unroll
-        for (int n = 0; n < COUNT; ++n)
-            v[n] = __builtin_amdgcn_raw_buffer_load_b128(b, src.at(r + n * (N / TL::NCH), c), 0, 0);
-    }
-    __device__ __forceinline__ void store(u4v* tile, int tid) const {
-        const int c = tid % TL::NCH, r = tid / TL::NCH;
-#pragma unroll
-        for (int n = 0; n < COUNT; ++n) tile[TL::slot(r + n * (N / TL::NCH), c)] = v[n];
-    }
-};
-
 // One tile of R rows straight from memory to LDS, by the waves of a workgroup together: an
 // instruction brings 64 chunks to consecutive slots, and each lane fetches the chunk that
 // belongs in its slot.  Out of range (past the last row, past D) comes as zeros.  Inline
