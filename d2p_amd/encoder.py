@@ -126,7 +126,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         key = seed & (2 ** 64 - 1)
         key -= (key >> 63) << 64            # as a signed 64-bit number
     if scale is None:
-        scale = q.shape[-1] ** -0.5
+        scale = max(q.shape[-1], 1) ** -0.5
     return torch.ops.d2p_amd.attention(q, k, v, lengths, causal, float(scale), bias, buckets,
                                        float(dropout), key, key_tensor)
 
@@ -153,8 +153,15 @@ class SequenceAttention(nn.Module):
                  num_buckets: int = 0, max_distance: int = 128, max_length: int = 4096,
                  rope_base: float = 10000.0, eps: float = 1e-6):
         super().__init__()
+        if heads < 1 or (kv_heads is not None and (kv_heads < 1 or heads % kv_heads)):
+            raise ValueError(f"heads must be a positive multiple of kv_heads, got {heads} and "
+                             f"{kv_heads}")
+        if head_dim is None and dim % heads:
+            raise ValueError(f"dim {dim} does not divide into {heads} heads; give head_dim")
         self.heads, self.kv_heads = heads, heads if kv_heads is None else kv_heads
         self.head_dim = dim // heads if head_dim is None else head_dim
+        if self.head_dim % 8 or not 8 <= self.head_dim <= 128:
+            raise ValueError(f"head_dim must be a multiple of 8 from 8 to 128, got {self.head_dim}")
         self.causal, self.dropout, self.eps = causal, dropout, eps
         self.qkv = nn.Linear(dim, (heads + 2 * self.kv_heads) * self.head_dim, bias=False)
         self.out = nn.Linear(heads * self.head_dim, dim, bias=False)
@@ -178,9 +185,8 @@ class SequenceAttention(nn.Module):
         return q, k, v
 
     def _attend(self, q, k, v, lengths, dropout=0.0, seed=None):
-        o = attention(q, k, v, lengths, causal=self.causal, bias=self.bias, buckets=self.buckets,
-                      dropout=dropout, seed=seed)
-        return self.out(o.flatten(2))
+        return attention(q, k, v, lengths, causal=self.causal, bias=self.bias,
+                         buckets=self.buckets, dropout=dropout, seed=seed).flatten(2)
 
     def forward(self, x: torch.Tensor, lengths: Optional[torch.Tensor] = None,
                 seed: Union[int, torch.Tensor, None] = None) -> torch.Tensor:
@@ -192,7 +198,7 @@ class SequenceAttention(nn.Module):
         p = self.dropout if self.training else 0.0
         if p and seed is None:
             seed = torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), device=x.device)
-        return self._attend(q, k, v, lengths, p, seed)
+        return self.out(self._attend(q, k, v, lengths, p, seed))
 
     def new_cache(self, batch: int, max_length: int, dtype=None) -> KeyValueCache:
         like = self.qkv.weight
@@ -204,15 +210,20 @@ class SequenceAttention(nn.Module):
     @torch.no_grad()
     def step(self, x: torch.Tensor, cache: KeyValueCache) -> torch.Tensor:
         """New tokens x [B, n, dim] of each sequence: their keys and values go into the cache,
-        whose lengths grow by n, and each attends to all before it."""
+        whose lengths grow by n, and each attends to all before it.  The host does not know
+        the lengths, so nothing waits: a sequence that outgrows its cache comes back NaN, in
+        that call and all later ones."""
         if not self.causal:
             raise ValueError("step() needs a causal layer")
-        n = x.shape[1]
+        n, room = x.shape[1], cache.keys.shape[1]
+        if n > room:
+            raise ValueError(f"{n} tokens do not fit a cache of {room}")
         at = cache.lengths[:, None] + torch.arange(n, dtype=torch.int32, device=x.device)
         q, k, v = self._project(x, at)
-        where = at.long()[:, :, None, None].expand_as(k)
+        where = at.long().clamp(max=room - 1)[:, :, None, None].expand_as(k)
         cache.keys.scatter_(1, where, k.to(cache.keys.dtype))
         cache.values.scatter_(1, where, v.to(cache.values.dtype))
         cache.lengths.add_(n)
         lengths = torch.stack((torch.full_like(cache.lengths, n), cache.lengths), 1)
-        return self._attend(q, cache.keys, cache.values, lengths)
+        o = self._attend(q.to(cache.keys.dtype), cache.keys, cache.values, lengths)
+        return self.out(o.to(q.dtype))

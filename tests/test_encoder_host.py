@@ -229,6 +229,10 @@ def test_python_layer_checks():
     assert m.qkv.weight.shape == (8 * 8, 32)
     with pytest.raises(ValueError, match="causal"):
         m.step(torch.randn(1, 1, 32), m.new_cache(1, 8))
+    for args, match in (((32, 5), "divide"), ((32, 4, 3), "multiple"), ((32, 0), "multiple"),
+                        ((48, 4), "head_dim"), ((32, 4, 2, 136), "head_dim")):
+        with pytest.raises(ValueError, match=match):
+            d2p_amd.SequenceAttention(*args)
 
 
 def test_philox_known_answer():

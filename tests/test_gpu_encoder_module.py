@@ -100,6 +100,24 @@ def test_cache_gives_what_the_whole_sequence_gives(cuda):
     assert (whole - parts).abs().max() <= 1e-5 and cache.lengths.tolist() == [30, 30]
 
 
+def test_a_full_cache_says_so(cuda):
+    torch.manual_seed(6)
+    layer = d2p_amd.SequenceAttention(64, 4, causal=True).to(cuda).eval()
+    x = torch.randn(2, 6, 64, device=cuda)
+    cache = layer.new_cache(2, 8, torch.bfloat16)
+    cache.lengths.copy_(torch.tensor([0, 5], device=cuda))
+    first = layer.step(x[:, :3], cache)
+    assert first.dtype == torch.float32 and first.isfinite().all()
+    second = layer.step(x[:, :2], cache)          # the second sequence has no room left
+    assert second[0].isfinite().all() and second[1].isnan().all()
+    third = layer.step(x, cache)
+    assert third.isnan().all()
+    with pytest.raises(ValueError, match="do not fit"):
+        layer.step(torch.randn(2, 9, 64, device=cuda), cache)
+    with pytest.raises(ValueError, match="causal"):
+        d2p_amd.SequenceAttention(64, 4).to(cuda).step(x, cache)
+
+
 def test_layer_compiles(cuda):
     torch.manual_seed(5)
     layer = d2p_amd.SequenceAttention(64, 2, num_buckets=8, max_distance=16).to(cuda)
