@@ -317,9 +317,9 @@ attention_dq_kernel(BackwardArgs a) {
 //
 // Bound as the kernel over queries, with a fourth product.  dK and dV of 128 features of 16
 // bits take half of the 256 registers that two waves a SIMD leave each, K's fragments an
-// eighth: V's come from LDS there ([2, 4096, 16, 128] bfloat16 causal: 338 us, 813 TFLOP/s,
-// against 471 with them in the registers of one wave a SIMD, and 366 where eight waves share
-// the tiles of queries).
+// eighth: V's come from LDS there ([2, 4096, 16, 128] bfloat16 causal: 313 us, 878 TFLOP/s; when
+// this was chosen 338, against 471 with them in the registers of one wave a SIMD, and 366 where
+// eight waves share the tiles of queries).
 template <class T, int DP> struct Dkv {
     static constexpr int NW = 4, KEYS = 32 * NW;
     static constexpr bool WIDE = Tile<T, DP>::ROW >= 256;   // V in LDS
