@@ -73,12 +73,12 @@ __device__ __forceinline__ void add_bias_by_key(f16v& s, float c, const float* b
 // Shared by the waves of a workgroup: K and V tiles of 64 keys, two of each, which go to
 // LDS without passing through registers while the tiles before them are worked on.
 //
-// A wave takes QT tiles of 32 queries.  In one turn of its loop the matrix cores form the
+// A wave takes 32 queries.  In one turn of its loop the matrix cores form the
 // next tile's scores while its vector units take the exponentials of this one, and P V of
 // each half of the keys while they take those of the other half and the next maximum.  The
 // accumulators are scaled to a new maximum only when it has grown by more than 2^8 (a
 // branch that is soon rare); until then the old one is a reference as good.
-template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward {
+template <class T, int DP, int NW, bool BIAS, bool DROP> struct Forward {
     using TL = Tile<T, DP>;
     using E = Elem<T>;
     static constexpr int BK = 64, DT = DP / 32, TILE = TL::bytes(BK) / 16;
@@ -91,10 +91,10 @@ template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward 
     const float* bias;
     const Drop drop;
     int lane, h, wq, at0;
-    int at[QT], limit[QT];
-    u4v qf[QT][TL::STEPS];
-    f16v o[QT][DT] = {};
-    float m[QT], ref[QT], l[QT];
+    int at, limit;
+    u4v qf[TL::STEPS];
+    f16v o[DT] = {};
+    float m = -__builtin_inff(), ref = 0.0f, l = 0.0f;
     float c;
 
     __device__ __forceinline__ Forward(const ForwardArgs& a_, const Span& e, const Rows& qr,
@@ -104,151 +104,125 @@ template <class T, int DP, int QT, int NW, bool BIAS, bool DROP> struct Forward 
           h(lane_ >> 5), wq(wq_), at0(wq_ + e.off) {
         c = p.scale * LOG2E;
         const __amdgpu_buffer_rsrc_t r = qr.from(wq);
+        const int i = wq + (lane & 31);
+        at = i + e.off;
+        limit = e.limit(p, i);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int i = wq + 32 * t + (lane & 31);
-            at[t] = i + e.off;
-            limit[t] = e.limit(p, i);
-            m[t] = -__builtin_inff();
-            ref[t] = 0.0f;
-            l[t] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < TL::STEPS; ++s)
-                qf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(r, qr.at(i - wq, 2 * s + h), 0, 0);
-        }
+        for (int s = 0; s < TL::STEPS; ++s)
+            qf[s] = __builtin_amdgcn_raw_buffer_load_b128(r, qr.at(lane & 31, 2 * s + h), 0, 0);
     }
 
-    __device__ __forceinline__ void scores(f16v (&s)[2][QT], int buf, int ra) const {
+    __device__ __forceinline__ void scores(f16v (&s)[2], int buf, int ra) const {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
+            s[k] = f16v{};
 #pragma unroll
-            for (int t = 0; t < QT; ++t) s[k][t] = f16v{};
-#pragma unroll
-            for (int n = 0; n < TL::STEPS; ++n) {
-                const u4v kf = TL::frag(Ks + buf * TILE, 32 * k, n, ra);
-#pragma unroll
-                for (int t = 0; t < QT; ++t) s[k][t] = E::mma(kf, qf[t][n], s[k][t]);
-            }
+            for (int n = 0; n < TL::STEPS; ++n)
+                s[k] = E::mma(TL::frag(Ks + buf * TILE, 32 * k, n, ra), qf[n], s[k]);
         }
     }
 
     // Bias and mask of the tile from key j0 on, and its place against the reference.
-    __device__ __forceinline__ void settle(f16v (&s)[2][QT], int j0, bool full) {
+    __device__ __forceinline__ void settle(f16v (&s)[2], int j0, bool full) {
         const int R = p.max_distance;
         const float inf = __builtin_inff();
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+            if (BIAS) add_bias(s[k], c, bias, R, j0 + 32 * k, at0, at, lane);
+            if (!full) {
+                const int left = limit - (j0 + 32 * k + 4 * h);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                if (BIAS)
-                    add_bias(s[k][t], c, bias, R, j0 + 32 * k, at0 + 32 * t, at[t], lane);
-                if (!full) {
-                    const int left = limit[t] - (j0 + 32 * k + 4 * h);
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        s[k][t][v] = 8 * (v >> 2) + (v & 3) < left ? s[k][t][v] : -inf;
-                }
+                for (int v = 0; v < 16; ++v)
+                    s[k][v] = 8 * (v >> 2) + (v & 3) < left ? s[k][v] : -inf;
             }
-        bool grown = false;
-        float top[QT];
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            float x = s[0][t][0];
-#pragma unroll
-            for (int v = 1; v < 32; ++v) x = fmaxf(x, s[v >> 4][t][v & 15]);
-            top[t] = both_max(x) * (BIAS ? 1.0f : c);
-            grown |= top[t] > m[t] + 8.0f;
         }
-        if (__any(grown)) {
+        float top = s[0][0];
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                const float to = fmaxf(m[t], top[t]);
-                const float f = to > m[t] ? exp2_(m[t] - to) : 1.0f;   // 0 from -inf
-                m[t] = to;
-                ref[t] = to == -inf ? 0.0f : to - FORWARD_SHIFT<T>;
-                l[t] *= f;
+        for (int v = 1; v < 32; ++v) top = fmaxf(top, s[v >> 4][v & 15]);
+        top = both_max(top) * (BIAS ? 1.0f : c);
+        if (__any(top > m + 8.0f)) {
+            const float to = fmaxf(m, top);
+            const float f = to > m ? exp2_(m - to) : 1.0f;   // 0 from -inf
+            m = to;
+            ref = to == -inf ? 0.0f : to - FORWARD_SHIFT<T>;
+            l *= f;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) o[t][d] *= f;
-            }
+            for (int d = 0; d < DT; ++d) o[d] *= f;
         }
     }
 
     // exponentials of half k of a tile: P, ready for the matrix cores
-    __device__ __forceinline__ void weights(const f16v (&s)[2][QT], int k, int j0,
-                                            u4v (&pf)[QT][TL::FRAGS]) {
+    __device__ __forceinline__ void weights(const f16v (&s)[2], int k, int j0,
+                                            u4v (&pf)[TL::FRAGS]) {
+        float x[16];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            float x[16];
+        for (int v = 0; v < 16; ++v) {
+            x[v] = exp2_(BIAS ? s[k][v] - ref : fmaf(s[k][v], c, -ref));
+            l += x[v];
+        }
+        u4v kw;
+        if (DROP) kw = drop.by_query(wq, j0 + 32 * k, lane);
+        if (DROP && sizeof(T) == 4) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                x[v] = exp2_(BIAS ? s[k][t][v] - ref[t] : fmaf(s[k][t][v], c, -ref[t]));
-                l[t] += x[v];
-            }
-            u4v kw;
-            if (DROP) kw = drop.by_query(wq + 32 * t, j0 + 32 * k, lane);
-            if (DROP && sizeof(T) == 4) {
+            for (int v = 0; v < 16; ++v) x[v] = drop.keeps(kw, v) ? x[v] : 0.0f;
+        }
+        // P in the type of V: its rounding is that of one factor of each product
 #pragma unroll
-                for (int v = 0; v < 16; ++v) x[v] = drop.keeps(kw, v) ? x[v] : 0.0f;
-            }
-            // P in the type of V: its rounding is that of one factor of each product
-#pragma unroll
-            for (int f = 0; f < TL::FRAGS; ++f) {
-                pf[t][f] = E::pack(x + TL::PER * f);
-                if (DROP && sizeof(T) == 2) pf[t][f] = drop.keep16(pf[t][f], kw, f);
-            }
+        for (int f = 0; f < TL::FRAGS; ++f) {
+            pf[f] = E::pack(x + TL::PER * f);
+            if (DROP && sizeof(T) == 2) pf[f] = drop.keep16(pf[f], kw, f);
         }
     }
 
-    __device__ __forceinline__ void values(const u4v (&pf)[QT][TL::FRAGS], int k, int buf, int ca) {
+    __device__ __forceinline__ void values(const u4v (&pf)[TL::FRAGS], int k, int buf, int ca) {
 #pragma unroll
         for (int f = 0; f < TL::FRAGS; ++f)
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const u4v vf = TL::frag_t(Vs + buf * TILE, 32 * k, 32 * d, f, ca);
-#pragma unroll
-                for (int t = 0; t < QT; ++t) o[t][d] = E::mma(vf, pf[t][f], o[t][d]);
-            }
+            for (int d = 0; d < DT; ++d)
+                o[d] = E::mma(TL::frag_t(Vs + buf * TILE, 32 * k, 32 * d, f, ca), pf[f], o[d]);
     }
 
     __device__ __forceinline__ void store(const Span& e, int b, int hq, int bh) {
         const int D = p.D;
         const float nan = __builtin_nanf("");
+        const int i = wq + (lane & 31);
+        const float sum = both_sum(l);
+        if (i >= p.Lq) return;
+        // no key: zeros, whatever the accumulators hold
+        const bool none = i >= e.nq || !(sum != 0.0f);
+        const float f = (DROP ? drop.scale : 1.0f) / sum;
+        char* row = (char*)a.out + (((long long)b * p.Lq + i) * p.Hq + hq) * D * (long long)sizeof(T);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int i = wq + 32 * t + (lane & 31);
-            const float sum = both_sum(l[t]);
-            if (i >= p.Lq) continue;
-            // no key: zeros, whatever the accumulators hold
-            const bool none = i >= e.nq || !(sum != 0.0f);
-            const float f = (DROP ? drop.scale : 1.0f) / sum;
-            char* row = (char*)a.out +
-                        (((long long)b * p.Lq + i) * p.Hq + hq) * D * (long long)sizeof(T);
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int g = 0; g < 4; ++g) {
+                const int d0 = 32 * d + 8 * g + 4 * h;
+                float y[4];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int d0 = 32 * d + 8 * g + 4 * h;
-                    float y[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        y[r] = e.bad ? nan : none ? 0.0f : o[t][d][4 * g + r] * f;
-                    if (d0 < D) E::store4(row + d0 * (int)sizeof(T), y);
-                }
-            if (h == 0) {
-                const long long n = (long long)p.B * p.Hq * p.Lq, x = (long long)bh * p.Lq + i;
-                a.stats[x] = e.bad ? nan : none ? -__builtin_inff() : m[t];
-                a.stats[n + x] = none ? 0.0f : log2_(sum) - FORWARD_SHIFT<T>;
+                for (int r = 0; r < 4; ++r) y[r] = e.bad ? nan : none ? 0.0f : o[d][4 * g + r] * f;
+                if (d0 < D) E::store4(row + d0 * (int)sizeof(T), y);
             }
+        if (h == 0) {
+            const long long n = (long long)p.B * p.Hq * p.Lq, x = (long long)bh * p.Lq + i;
+            a.stats[x] = e.bad ? nan : none ? -__builtin_inff() : m;
+            a.stats[n + x] = none ? 0.0f : log2_(sum) - FORWARD_SHIFT<T>;
         }
     }
 };
 
-template <class T, int DP, int QT, int NW, bool BIAS, bool DROP>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) * DP >= 512 ? 1 : 2)
+// Waves a SIMD that the registers are dealt for: the vector work of bias and dropout together
+// gains by a third one at 64 features of 16 bits ([8, 2048, 8, 64] bfloat16 causal: 85 -> 75 us, two
+// registers in scratch); dropout alone loses by it (nine in scratch, 65 -> 71 us).
+template <class T, int DP, bool BIAS, bool DROP> constexpr int forward_waves() {
+    return sizeof(T) * DP >= 512 ? 1 : sizeof(T) * DP == 128 && BIAS && DROP ? 3 : 2;
+}
+
+template <class T, int DP, int NW, bool BIAS, bool DROP>
+__global__ void __launch_bounds__(64 * NW, (forward_waves<T, DP, BIAS, DROP>()))
 attention_forward_kernel(ForwardArgs a) {
-    using F = Forward<T, DP, QT, NW, BIAS, DROP>;
+    using F = Forward<T, DP, NW, BIAS, DROP>;
     using TL = Tile<T, DP>;
-    constexpr int BK = F::BK, ROWS = 32 * QT * NW;
+    constexpr int BK = F::BK, ROWS = 32 * NW;
     extern __shared__ __align__(16) u4v sm[];
     u4v* Ks = sm;
     u4v* Vs = sm + 2 * F::TILE;
@@ -274,24 +248,24 @@ attention_forward_kernel(ForwardArgs a) {
     dv.init(vr, wave, lane);
     if (tiles > 0) dk.issue(kr, 0, Ks, wave);
     if (BIAS) load_bias<T>(bias, p, hq, tid, 64 * NW);
-    F f(a, e, qr, sm, bias, bh, q0 + 32 * QT * wave, lane);
+    F f(a, e, qr, sm, bias, bh, q0 + 32 * wave, lane);
     // keys that all, that any of the wave's queries see
     const int wave_full = e.limit(p, f.wq);
-    const int wave_end = f.wq < e.nq ? e.limit(p, min(f.wq + 32 * QT, e.nq) - 1) : 0;
+    const int wave_end = f.wq < e.nq ? e.limit(p, min(f.wq + 32, e.nq) - 1) : 0;
     if (tiles > 0) {
-        f16v s0[2][QT], s1[2][QT];
+        f16v s0[2], s1[2];
         wait_dma();
         __syncthreads();
         dv.issue(vr, 0, Vs, wave);
         if (tiles > 1) dk.issue(kr, BK, Ks + F::TILE, wave);
         f.scores(s0, 0, ra);
         f.settle(s0, 0, BK <= wave_full);
-        auto turn = [&](f16v (&now)[2][QT], f16v (&next)[2][QT], int n, int buf) {
+        auto turn = [&](f16v (&now)[2], f16v (&next)[2], int n, int buf) {
             wait_dma();
             meet();
             if (n + 1 < tiles) dv.issue(vr, (n + 1) * BK, Vs + (buf ^ 1) * F::TILE, wave);
             if (n + 2 < tiles) dk.issue(kr, (n + 2) * BK, Ks + buf * F::TILE, wave);
-            u4v p0[QT][TL::FRAGS], p1[QT][TL::FRAGS];
+            u4v p0[TL::FRAGS], p1[TL::FRAGS];
             if (n * BK >= wave_end) return;
             // (float32 by 128: [4, 1024, 8, 128] 207 -> 169 us; 16 bits by 128 have the registers,
             // and lose by it: [2, 8192, 16, 128] 1045 -> 1240 us)
@@ -313,14 +287,14 @@ attention_forward_kernel(ForwardArgs a) {
     f.store(e, b, hq, bh);
 }
 
-template <class T, int DP, int QT, int NW, bool BIAS, bool DROP>
+template <class T, int DP, int NW, bool BIAS, bool DROP>
 int launch_forward_as(const ForwardArgs& a, hipStream_t st) {
-    auto kernel = attention_forward_kernel<T, DP, QT, NW, BIAS, DROP>;
-    const int lds = Forward<T, DP, QT, NW, BIAS, DROP>::LDS +
+    auto kernel = attention_forward_kernel<T, DP, NW, BIAS, DROP>;
+    const int lds = Forward<T, DP, NW, BIAS, DROP>::LDS +
                     (BIAS ? (2 * a.p.max_distance + 1) * 4 : 0);
     static LdsAllowed known;
     D2P_TRY(allow_lds((const void*)kernel, known));
-    const long long n = (long long)a.p.B * a.p.Hq * cdiv(a.p.Lq, 32 * QT * NW);
+    const long long n = (long long)a.p.B * a.p.Hq * cdiv(a.p.Lq, 32 * NW);
     D2P_REQUIRE(n <= 0x7fffffffLL, "too many query blocks");
     if (n == 0) return D2P_OK;
     D2P_LAUNCH("attention_forward", kernel, dim3((unsigned)n), dim3(64 * NW), lds, st, a);
@@ -336,8 +310,8 @@ template <class T, int DP, bool BIAS, bool DROP>
 int launch_forward_shape(const ForwardArgs& a, hipStream_t st) {
     if constexpr (DP == 128 && sizeof(T) == 2)
         if ((long long)a.p.B * a.p.Hq * cdiv(a.p.Lq, 256) >= 2LL * device_cus())
-            return launch_forward_as<T, DP, 1, 8, BIAS, DROP>(a, st);
-    return launch_forward_as<T, DP, 1, 4, BIAS, DROP>(a, st);
+            return launch_forward_as<T, DP, 8, BIAS, DROP>(a, st);
+    return launch_forward_as<T, DP, 4, BIAS, DROP>(a, st);
 }
 
 template <class T, int DP> int launch_forward_dp(const ForwardArgs& a, hipStream_t st) {
