@@ -130,6 +130,30 @@ def test_ragged_and_empty(cuda, dtype, causal):
         assert (got["out"][4, :57] == 0).all() and (got["out"][4, 57:] != 0).any()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_a_filled_card(cuda, dtype):
+    """Enough blocks of queries for the wider workgroups that wide heads take then."""
+    ls = lens(cuda, (520, 70), (257, 33), (1, 70), (519, 0))
+    both(inputs(12, 4, 520, 70, 64, 4, 128, dtype, cuda), lengths=ls)
+    both(inputs(13, 4, 520, 70, 64, 64, 128, dtype, cuda, 8, 16), causal=True, drop=40, seed=9)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_queries_use_nothing_past_the_lengths(cuda, D, dtype):
+    ls = lens(cuda, (2, 3000), (1, 17), (2, 1), (2, 0), (0, 50), (1, 2049))
+    q, k, v, _, bias, where = inputs(14, len(ls), 2, 3000, 4, 2, D, dtype, cuda, 8, 16)
+    for causal in (False, True):
+        want = run(q, k, v, None, ls, causal, None, bias, where)["out"]
+        q2, k2, v2 = q.clone(), k.clone(), v.clone()
+        for b, (nq, nk) in enumerate(ls.tolist()):
+            q2[b, nq:] = float("inf")
+            k2[b, nk:] = float("nan")
+            v2[b, nk:] = float("-inf")
+        assert torch.equal(run(q2, k2, v2, None, ls, causal, None, bias, where)["out"], want)
+        assert (want[3] == 0).all() and (want[4] == 0).all() and want.isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_bias_that_masks(cuda, dtype):
     """-inf hides pairs, and a row of nothing else is zeros; the type's lowest value does not
