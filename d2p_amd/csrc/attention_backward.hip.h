@@ -130,8 +130,12 @@ attention_dq_kernel(BackwardArgs a) {
     }
     if (BIAS) load_bias<T>(bias, p, hq, tid, 64 * NW);
     if (DBIAS) {
-        for (int t = tid; t < NW * span; t += 64 * NW) hists[t] = 0.0f;
+        // each wave its own, which no other reads before the barrier of the join: a block without
+        // tiles meets no barrier ahead of that
+        for (int t = lane; t < span; t += 64) hists[wave * span + t] = 0.0f;
         for (int t = lane; t < BiasSums::TILE; t += 64) tile[t] = 0.0f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 
     u4v qf[TL::STEPS], gf[TL::STEPS];

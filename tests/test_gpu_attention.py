@@ -393,3 +393,20 @@ def test_empty_tensors(cuda):
         assert got["out"].shape == (B, Lq, 2, 16)
         if B == 0 or Lq == 0 or Lk == 0:
             assert all((x == 0).all() for x in got.values())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("R", [16, 130, 1024])
+def test_bias_gradient_beside_blocks_without_keys(cuda, R, causal, dtype):
+    """Blocks of queries past nq, of elements without keys and (causal) before the first key add
+    nothing to the bias's gradient, whatever the workgroups before them left in LDS."""
+    ls = lens(cuda, (520, 140), (3, 140), (100, 0), (0, 0), (520, 1), (0, 140), (130, 7), (520, 0))
+    args = inputs(23, len(ls), 520, 140, 2, 1, 64, dtype, cuda, 12, R)
+    got = both(args, lengths=ls, causal=causal)
+    for _ in range(5):
+        again = run(*args[:4], ls, causal, None, *args[4:])
+        assert all(torch.equal(got[n], again[n]) for n in got)
+    # nothing but such blocks
+    ls = lens(cuda, *[(0, 140), (520, 0), (0, 0), (130, 0)] * 2)
+    assert all((x == 0).all() for x in run(*args[:4], ls, causal, None, *args[4:]).values())
