@@ -133,15 +133,15 @@ __global__ void __launch_bounds__(256) attention_few_kernel(FewArgs fa) {
             top = fmaxf(top, x[v]);
         }
         top = fmaxf(m, both_max(top));
-        const float ref = (top == -__builtin_inff() ? 0.0f : top) - FORWARD_SHIFT<T>;
-        const float old = exp2_(m - (FORWARD_SHIFT<T> + ref));
+        const float ref = top == -__builtin_inff() ? 0.0f : top;
+        const float old = exp2_(m - ref);
         m = top;
         l *= old;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= old;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-            x[v] = exp2_(x[v] - ref);
+            x[v] = exp2_(shifted<T>(x[v] - ref));
             l += x[v];
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -144,7 +144,8 @@ template <class T, int DP, int NW, bool BIAS, bool DROP> struct Forward {
             const float to = fmaxf(m, top);
             const float f = to > m ? exp2_(m - to) : 1.0f;   // 0 from -inf
             m = to;
-            ref = to == -inf ? 0.0f : to - FORWARD_SHIFT<T>;
+            // (without a bias the shift is part of it, rounded like the scores themselves)
+            ref = to == -inf ? 0.0f : BIAS ? to : to - FORWARD_SHIFT<T>;
             l *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
@@ -157,7 +158,7 @@ template <class T, int DP, int NW, bool BIAS, bool DROP> struct Forward {
         float x[16];
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-            x[v] = exp2_(BIAS ? s[k][v] - ref : fmaf(s[k][v], c, -ref));
+            x[v] = exp2_(BIAS ? shifted<T>(s[k][v] - ref) : fmaf(s[k][v], c, -ref));
             l += x[v];
         }
         u4v kw;

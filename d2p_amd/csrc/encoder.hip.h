@@ -280,6 +280,12 @@ template <class T> constexpr int FORWARD_SHIFT = NARROW<T> ? 7 : 0;
 template <class T> constexpr int BACKWARD_SHIFT = NARROW<T> ? 12 : 0;
 template <class T> constexpr int DS_SHIFT = NARROW<T> ? 2 : 0;
 
+// a score less its row's reference, shifted for the forward.  The difference comes first: taken
+// off the reference, the shift would be rounded away beside a bias of the size of 2^24 and more.
+template <class T> __device__ __forceinline__ float shifted(float d) {
+    return FORWARD_SHIFT<T> ? d + FORWARD_SHIFT<T> : d;
+}
+
 // 2^n, n from -126 to 127
 __device__ __forceinline__ float pow2(int n) { return bits<float>((unsigned)(127 + n) << 23); }
 // the least e with |x| < 2^e; -100 for zero, 0 for infinity and NaN

@@ -410,3 +410,32 @@ def test_bias_gradient_beside_blocks_without_keys(cuda, R, causal, dtype):
     # nothing but such blocks
     ls = lens(cuda, *[(0, 140), (520, 0), (0, 0), (130, 0)] * 2)
     assert all((x == 0).all() for x in run(*args[:4], ls, causal, None, *args[4:]).values())
+
+
+HALF_SIZES = [(2, 40, 40, 2, 2, 32), (1, 3, 400, 4, 2, 64), (1, 3, 1500, 2, 1, 64), (1, 200, 130, 2, 1, 128)]
+
+
+@pytest.mark.parametrize("low", [-2e7, -1e8, -1e9, torch.finfo(F32).min])
+@pytest.mark.parametrize("size", HALF_SIZES, ids=str)
+def test_half_beside_low_biases_in_32_bits(cuda, size, low):
+    """Rows whose every bias is the same low number keep probabilities that sum to one in the
+    backward pass, from either forward.  So the sum of dv over the keys is that of the gradients:
+    P and dv are rounded to half once each, the statistics are good to 2^-18.  Below -2^29 a score
+    adds nothing to its bias, and everything is what equal scores give."""
+    q, k, v, g, _, where = inputs(21, *size, F16, cuda, 3, 20)
+    B, Lq, Lk, Hq, Hkv, D = size
+    bias = torch.full((3, Hq), low, device=cuda)
+    got = run(q, k, v, g, bias=bias, buckets=where)
+    assert all(x.isfinite().all() for x in got.values())
+    u = ref.U[F16]
+    have = got["dv"].double().sum(1)
+    join = lambda x: x.double().sum(1).view(B, Hkv, Hq // Hkv, D).sum(2)  # noqa: E731
+    bound = (2 * u + 2.0 ** -18) * join(g.abs()) + Lk * ref.TINY[F16]
+    assert ((have - join(g)).abs() <= bound).all()
+    if low < -2.0 ** 29:
+        tiny = 2.0 ** -40          # a scale that leaves the scores equal in 64 bits, undone
+        want, err = ref.attention(q, k, v, g, scale=tiny, bias=bias * 0, buckets=where)
+        for n in ("dq", "dk"):
+            f = D ** -0.5 / tiny
+            want[n], err[n] = want[n] * f, (err[n] - ref.TINY[F16]) * f + ref.TINY[F16]
+        check(got, want, err)
