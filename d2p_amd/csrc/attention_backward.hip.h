@@ -192,7 +192,9 @@ attention_dq_kernel(BackwardArgs a) {
     // keys that all, that any of the wave's queries see
     const int wave_full = e.limit(p, wq);
     const int wave_end = wq < e.nq ? e.limit(p, min(wq + 32, e.nq) - 1) : 0;
-    const int limit = e.limit(p, i);
+    // (rows past the last see none: a bias of distances that only they have may be NaN)
+    const int limit = !BIAS || i < e.nq ? e.limit(p, i) : 0;
+    const int unmasked = !BIAS || wq + 32 <= e.nq ? wave_full : 0;
 
     const int ra = TL::row_at(lane), ca = TL::col_at(lane);
     // probabilities x and kept gradients dp (not yet scaled) of 32 keys of a tile
@@ -205,7 +207,7 @@ attention_dq_kernel(BackwardArgs a) {
         for (int n = 0; n < TL::STEPS; ++n)
             dp = Elem<T>::mma(TL::frag(vt, 32 * t, n, ra), gf[n], dp);
         if (BIAS) add_bias(s, c, bias, R, jt, wq + e.off, at, lane);
-        if (jt + 32 > wave_full) {
+        if (jt + 32 > unmasked) {
             const int left = limit - (jt + 4 * h);
 #pragma unroll
             for (int v = 0; v < 16; ++v)
@@ -485,6 +487,13 @@ attention_dkv_kernel(BackwardArgs a) {
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
                         s[v] = 8 * (v >> 2) + (v & 3) >= from ? s[v] : -__builtin_inff();
+                }
+                if (BIAS && it + 32 > e.nq) {
+                    // as in the kernel over queries
+                    const int left = e.nq - (it + 4 * h);
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        s[v] = 8 * (v >> 2) + (v & 3) < left ? s[v] : -__builtin_inff();
                 }
                 const u4v kw = DROP ? drop.by_key(it, wk, lane) : u4v{};
 #pragma unroll

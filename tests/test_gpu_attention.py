@@ -439,3 +439,28 @@ def test_half_beside_low_biases_in_32_bits(cuda, size, low):
             f = D ** -0.5 / tiny
             want[n], err[n] = want[n] * f, (err[n] - ref.TINY[F16]) * f + ref.TINY[F16]
         check(got, want, err)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_bias_of_distances_that_only_padded_queries_have(cuda, causal, D, dtype):
+    """NaN, infinity or a bucket that does not exist, at distances that no pair within the
+    lengths has, changes no bit; that bucket's gradient is zero."""
+    nq, nk = 40, 60
+    q, k, v, g, bias, _ = inputs(22, 1, 100, 60, 2, 1, D, dtype, cuda, 2, 64)
+    ls = lens(cuda, (nq, nk))
+    lowest = -nq + 1 - (nk - nq if causal else 0)         # the smallest j - at_i within the lengths
+    where = torch.tensor([int(d < lowest) for d in range(-64, 65)], dtype=torch.int32, device=cuda)
+    if causal:
+        # ahead of a query no pair is seen, but padded queries of the same tile see those
+        where[64 + 1:] = 1
+    bias[1] = 0
+    want = run(q, k, v, g, ls, causal, None, bias, where)
+    assert (want["dbias"][1] == 0).all()
+    gone = where.clone()
+    gone[where == 1] = 7
+    for value, place in ((float("nan"), where), (float("inf"), where), (0.0, gone)):
+        bias[1] = value
+        got = run(q, k, v, g, ls, causal, None, bias, place)
+        assert all(torch.equal(got[n], want[n]) for n in want), value
