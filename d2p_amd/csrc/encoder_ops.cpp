@@ -240,6 +240,13 @@ struct BelowAutograd {
     }
 };
 
+// Forward-mode derivatives are not implemented: a tangent raises, with and without gradients.
+void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name,
+                                    " does not support forward AD");
+}
+
 OptTensor saved(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
 class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
@@ -264,6 +271,7 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const auto s = ctx->get_saved_variables();
         const bool bias_grad = ctx->saved_data["bias"].toBool();
+        no_tangents("attention's backward", {&grads[0]});
         BelowAutograd below;
         static auto op = operator_handle<decltype(attention_backward)>("d2p_amd::attention_backward");
         auto [dq, dk, dv, db] = op.call(
@@ -295,6 +303,7 @@ Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v,
                           const OptTensor& bias, const OptTensor& buckets, double dropout,
                           int64_t seed, const OptTensor& seed_tensor) {
     const Tensor b = bias.value_or(Tensor());
+    no_tangents("attention", {&q, &k, &v, &b});
     if (differentiates({&q, &k, &v, &b}))
         return AttentionFunction::apply(q, k, v, lengths, causal, scale, bias, buckets, dropout,
                                         seed, seed_tensor);
@@ -462,6 +471,7 @@ class QkNormRopeFunction : public torch::autograd::Function<QkNormRopeFunction> 
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const auto s = ctx->get_saved_variables();
         const bool weights = ctx->saved_data["weights"].toBool();
+        no_tangents("qk_norm_rope's backward", {&grads[0], &grads[1]});
         BelowAutograd below;
         static auto op =
             operator_handle<decltype(qk_norm_rope_backward)>("d2p_amd::qk_norm_rope_backward");
@@ -482,6 +492,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope_autograd(const Tensor& q, const Tensor& 
                                                  const Tensor& sin, const OptTensor& positions,
                                                  double eps, bool interleaved) {
     const Tensor wq = q_weight.value_or(Tensor()), wk = k_weight.value_or(Tensor());
+    no_tangents("qk_norm_rope", {&q, &k, &wq, &wk, &cos, &sin});
     TORCH_CHECK(!differentiates({&cos, &sin}), "cos and sin do not take gradients");
     if (differentiates({&q, &k, &wq, &wk})) {
         auto r = QkNormRopeFunction::apply(q, k, q_weight, k_weight, cos, sin, positions, eps,

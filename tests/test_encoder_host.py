@@ -261,3 +261,40 @@ def test_oracle_gradient_against_differences():
 
         h = 1e-5     # h^2 f''' / 6 and 1e-16 f / h are both below 1e-9
         assert abs((f(h) - f(-h)) / (2 * h) - (res[name] * d).sum()) < 1e-8
+
+
+def test_forward_mode_raises():
+    """No operator has a derivative in forward mode: a tangent raises, on whichever input, and is
+    never dropped (meta tensors: the operators' autograd layer without their kernels)."""
+    import torch.autograd.forward_ad as fwd
+    m = dict(device="meta")
+    q, k = torch.empty(2, 5, 4, 16, **m), torch.empty(2, 7, 2, 16, **m)
+    bias, where = torch.empty(3, 4, **m), torch.empty(5, dtype=torch.int32, **m)
+    w, cos = torch.empty(16, **m), torch.empty(5, 8, **m)
+
+    def attend(q, k, v, b):
+        return d2p_amd.attention(q, k, v, bias=b, buckets=where)
+
+    def norm(q, k, wq, wk, c, s):
+        return d2p_amd.qk_norm_rope(q, k, wq, wk, c, s)
+
+    for f, args in ((attend, (q, k, k, bias)), (norm, (q, q[:, :, :2], w, w, cos, cos))):
+        f(*args)
+        for n, x in enumerate(args):
+            def of(y):
+                return f(*args[:n], y, *args[n + 1:])
+            with pytest.raises(RuntimeError, match="forward AD"):
+                torch.func.jvp(of, (x,), (torch.ones_like(x),))
+            for grad in (False, True):
+                with fwd.dual_level(), pytest.raises(RuntimeError, match="forward AD"):
+                    of(fwd.make_dual(x.detach().requires_grad_(grad), torch.ones_like(x)))
+        with torch.no_grad(), fwd.dual_level(), pytest.raises(RuntimeError, match="forward AD"):
+            of(fwd.make_dual(x, torch.ones_like(x)))
+        # nor has the backward pass
+        x = args[0].detach().requires_grad_()
+        out = f(x, *args[1:])
+        out = out if isinstance(out, torch.Tensor) else out[0]
+        g = torch.ones_like(out)
+        torch.autograd.grad(out, x, g, retain_graph=True)
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="forward AD"):
+            torch.autograd.grad(out, x, fwd.make_dual(g, g))
