@@ -176,6 +176,14 @@ class SequenceAttention(nn.Module):
             self.bias = nn.Parameter(torch.zeros(num_buckets, heads))
             self.buckets = relative_buckets(num_buckets, max_distance, not causal)
 
+    def _apply(self, fn, recurse=True):
+        # a layer moved to another type: the angles, which the kernels read in 32 bits, keep theirs
+        tables = self.cos, self.sin
+        super()._apply(fn, recurse)
+        if self.cos.dtype != torch.float32:
+            self.cos, self.sin = (t.to(self.cos.device) for t in tables)
+        return self
+
     def _project(self, x, positions):
         B, L, _ = x.shape
         qkv = self.qkv(x).view(B, L, self.heads + 2 * self.kv_heads, self.head_dim)

@@ -298,3 +298,14 @@ def test_forward_mode_raises():
         torch.autograd.grad(out, x, g, retain_graph=True)
         with fwd.dual_level(), pytest.raises(RuntimeError, match="forward AD"):
             torch.autograd.grad(out, x, fwd.make_dual(g, g))
+
+
+def test_layer_tables_stay_in_32_bits():
+    """Rotation tables are float32 whatever type the layer is moved to, and unrounded."""
+    want = d2p_amd.rope_tables(50, 8, 100.0)
+    for moves in ((torch.bfloat16,), (torch.float16, torch.float32), (torch.float64, torch.bfloat16)):
+        m = d2p_amd.SequenceAttention(32, 4, num_buckets=8, max_length=50, rope_base=100.0)
+        for to in moves:
+            m = m.to(to)
+        assert m.qkv.weight.dtype == m.bias.dtype == moves[-1] and m.buckets.dtype == torch.int32
+        assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip((m.cos, m.sin), want))

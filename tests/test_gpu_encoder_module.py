@@ -136,3 +136,23 @@ def test_example_learns(cuda):
         losses = example().train(steps=30, batch=16, length=64, autocast=autocast, report=lambda _: None)
         last = sum(losses[-5:]) / 5
         assert last < 0.6 and last < losses[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_layer_in_16_bits(cuda, dtype):
+    """A layer moved to 16 bits is its operators in 16 bits, with angles in 32."""
+    torch.manual_seed(7)
+    layer = d2p_amd.SequenceAttention(64, 4, 2, causal=True, num_buckets=8, max_distance=16)
+    torch.nn.init.normal_(layer.bias)
+    layer = layer.to(cuda).to(dtype).eval()
+    x = torch.randn(2, 30, 64, device=cuda, dtype=dtype)
+    q, k, v = layer.qkv(x).view(2, 30, 8, 16).split((4, 2, 2), 2)
+    q, k = d2p_amd.qk_norm_rope(q, k, layer.q_norm, layer.k_norm,
+                                *d2p_amd.rope_tables(30, 16, device=cuda))
+    o = d2p_amd.attention(q, k, v, causal=True, bias=layer.bias, buckets=layer.buckets)
+    got = layer(x)
+    assert got.dtype == dtype and torch.equal(got, layer.out(o.flatten(2)))
+    got.sum().backward()
+    assert all(p.grad.dtype == dtype and p.grad.isfinite().all() for p in layer.parameters())
+    cache = layer.new_cache(2, 30)
+    assert cache.keys.dtype == dtype and layer.step(x, cache).isfinite().all()
