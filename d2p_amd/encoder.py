@@ -193,7 +193,10 @@ class SequenceAttention(nn.Module):
         return q, k, v
 
     def _attend(self, q, k, v, lengths, dropout=0.0, seed=None):
-        return attention(q, k, v, lengths, causal=self.causal, bias=self.bias,
+        bias = self.bias
+        if bias is not None and bias.dtype not in (torch.float32, q.dtype):
+            bias = bias.float()     # (a 16-bit layer and a cache of another type)
+        return attention(q, k, v, lengths, causal=self.causal, bias=bias,
                          buckets=self.buckets, dropout=dropout, seed=seed).flatten(2)
 
     def forward(self, x: torch.Tensor, lengths: Optional[torch.Tensor] = None,

@@ -156,3 +156,20 @@ def test_layer_in_16_bits(cuda, dtype):
     assert all(p.grad.dtype == dtype and p.grad.isfinite().all() for p in layer.parameters())
     cache = layer.new_cache(2, 30)
     assert cache.keys.dtype == dtype and layer.step(x, cache).isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_cache_of_another_type(cuda, dtype):
+    """Tokens attend in the cache's type, with the bias's numbers as they are."""
+    torch.manual_seed(8)
+    layer = d2p_amd.SequenceAttention(64, 4, 2, causal=True, num_buckets=8, max_distance=16)
+    torch.nn.init.normal_(layer.bias)
+    layer = layer.to(cuda).to(dtype).eval()
+    x = torch.randn(2, 9, 64, device=cuda, dtype=dtype)
+    for of in (torch.float32, torch.float16, torch.bfloat16):
+        cache = layer.new_cache(2, 9, of)
+        got = layer.step(x, cache)
+        q, k, v = layer._project(x, None)
+        o = d2p_amd.attention(q.to(of), k.to(of), v.to(of), causal=True, bias=layer.bias.float(),
+                              buckets=layer.buckets)
+        assert got.dtype == dtype and torch.equal(got, layer.out(o.flatten(2).to(dtype)))
