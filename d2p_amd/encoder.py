@@ -223,7 +223,7 @@ class SequenceAttention(nn.Module):
         """New tokens x [B, n, dim] of each sequence: their keys and values go into the cache,
         whose lengths grow by n, and each attends to all before it.  The host does not know
         the lengths, so nothing waits: a sequence that outgrows its cache comes back NaN, in
-        that call and all later ones."""
+        that call and all later ones, and so does one whose length is below zero."""
         if not self.causal:
             raise ValueError("step() needs a causal layer")
         n, room = x.shape[1], cache.keys.shape[1]
@@ -231,10 +231,12 @@ class SequenceAttention(nn.Module):
             raise ValueError(f"{n} tokens do not fit a cache of {room}")
         at = cache.lengths[:, None] + torch.arange(n, dtype=torch.int32, device=x.device)
         q, k, v = self._project(x, at)
-        where = at.long().clamp(max=room - 1)[:, :, None, None].expand_as(k)
+        where = at.long().clamp(0, room - 1)[:, :, None, None].expand_as(k)
         cache.keys.scatter_(1, where, k.to(cache.keys.dtype))
         cache.values.scatter_(1, where, v.to(cache.values.dtype))
+        # n queries; -1, which attention answers with NaN, where the length is below zero
+        queries = cache.lengths >> 31 | n
         cache.lengths.add_(n)
-        lengths = torch.stack((torch.full_like(cache.lengths, n), cache.lengths), 1)
+        lengths = torch.stack((queries, cache.lengths), 1)
         o = self._attend(q.to(cache.keys.dtype), cache.keys, cache.values, lengths)
         return self.out(o.to(q.dtype))

@@ -173,3 +173,21 @@ def test_cache_of_another_type(cuda, dtype):
         o = d2p_amd.attention(q.to(of), k.to(of), v.to(of), causal=True, bias=layer.bias.float(),
                               buckets=layer.buckets)
         assert got.dtype == dtype and torch.equal(got, layer.out(o.flatten(2).to(dtype)))
+
+
+def test_lengths_below_zero_are_nan(cuda):
+    """A cache whose lengths somebody made negative: that sequence is NaN, its neighbours are
+    what they are without it, and nothing outside its own rows is written."""
+    torch.manual_seed(9)
+    layer = d2p_amd.SequenceAttention(64, 4, causal=True).to(cuda).eval()
+    x = torch.randn(3, 2, 64, device=cuda)
+    want_cache, cache = layer.new_cache(3, 8), layer.new_cache(3, 8)
+    want = layer.step(x, want_cache)
+    for wrong in (-1, -2, -7, -2 ** 31):
+        cache = layer.new_cache(3, 8)
+        cache.lengths[1] = wrong
+        got = layer.step(x, cache)
+        assert got[1].isnan().all(), wrong
+        for b in (0, 2):
+            assert torch.equal(got[b], want[b]) and torch.equal(cache.keys[b], want_cache.keys[b])
+            assert torch.equal(cache.values[b], want_cache.values[b])
