@@ -211,7 +211,14 @@ class SequenceAttention(nn.Module):
             seed = torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), device=x.device)
         return self.out(self._attend(q, k, v, lengths, p, seed))
 
+    def _check_room(self, room):
+        # past the tables a key would be NaN, and all that attend to it
+        if room > self.cos.shape[0]:
+            raise ValueError(f"a cache of {room} tokens exceeds the layer's max_length "
+                             f"{self.cos.shape[0]}")
+
     def new_cache(self, batch: int, max_length: int, dtype=None) -> KeyValueCache:
+        self._check_room(max_length)
         like = self.qkv.weight
         shape = (batch, max_length, self.kv_heads, self.head_dim)
         return KeyValueCache(torch.zeros(shape, dtype=dtype or like.dtype, device=like.device),
@@ -229,6 +236,7 @@ class SequenceAttention(nn.Module):
         n, room = x.shape[1], cache.keys.shape[1]
         if n > room:
             raise ValueError(f"{n} tokens do not fit a cache of {room}")
+        self._check_room(room)
         at = cache.lengths[:, None] + torch.arange(n, dtype=torch.int32, device=x.device)
         q, k, v = self._project(x, at)
         where = at.long().clamp(0, room - 1)[:, :, None, None].expand_as(k)

@@ -191,3 +191,15 @@ def test_lengths_below_zero_are_nan(cuda):
         for b in (0, 2):
             assert torch.equal(got[b], want[b]) and torch.equal(cache.keys[b], want_cache.keys[b])
             assert torch.equal(cache.values[b], want_cache.values[b])
+
+
+def test_cache_no_longer_than_the_tables(cuda):
+    layer = d2p_amd.SequenceAttention(64, 4, causal=True, max_length=16).to(cuda).eval()
+    with pytest.raises(ValueError, match="max_length"):
+        layer.new_cache(2, 17)
+    cache = layer.new_cache(2, 16)
+    assert layer.step(torch.randn(2, 16, 64, device=cuda), cache).isfinite().all()
+    longer = d2p_amd.KeyValueCache(*(torch.zeros(2, 17, 4, 16, device=cuda) for _ in range(2)),
+                                   torch.zeros(2, dtype=torch.int32, device=cuda))
+    with pytest.raises(ValueError, match="max_length"):
+        layer.step(torch.randn(2, 1, 64, device=cuda), longer)
