@@ -7,7 +7,7 @@
 namespace d2p_amd {
 namespace enc {
 
-int check_strides(const d2p_strides& s, int rows, int D, int dtype, const char* name) {
+static int check_strides(const d2p_strides& s, int rows, int D, int dtype, const char* name) {
     const int per = dtype == D2P_FLOAT32 ? 4 : 8;   // elements of 16 bytes
     if (s.batch % per || s.row % per || s.head % per) {
         set_last_error("%s: strides must be multiples of 16 bytes", name);
@@ -24,7 +24,8 @@ int check_strides(const d2p_strides& s, int rows, int D, int dtype, const char* 
     return D2P_OK;
 }
 
-int check_attention(const d2p_attention_params* p) {
+// Every argument of an attention call that the host can see.
+static int check_attention(const d2p_attention_params* p) {
     D2P_REQUIRE(p != nullptr, "null parameters");
     D2P_REQUIRE(p->dtype == D2P_FLOAT32 || p->dtype == D2P_FLOAT16 || p->dtype == D2P_BFLOAT16,
                 "unknown element type");

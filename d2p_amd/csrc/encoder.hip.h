@@ -274,7 +274,9 @@ __device__ __forceinline__ float both_sum(float x) {
 // probabilities by 2^FORWARD_SHIFT in the forward (at most 1 there) and 2^BACKWARD_SHIFT in
 // the backward; dS by 2^DS_SHIFT over the power of two at the largest gradient of the row
 // or head.  Without it keys of small probability lose bits to subnormal numbers, and
-// gradients of small magnitude vanish.
+// gradients of small magnitude vanish.  The other end of the range: dS is finite up to 2^14
+// times that power of two, which takes values of several hundred in step with the gradients
+// over all of 128 features.
 template <class T> constexpr bool NARROW = __is_same(T, _Float16);
 template <class T> constexpr int FORWARD_SHIFT = NARROW<T> ? 7 : 0;
 template <class T> constexpr int BACKWARD_SHIFT = NARROW<T> ? 12 : 0;
@@ -505,10 +507,6 @@ inline int allow_lds(const void* kernel, LdsAllowed& known) {
     if (keep) known.on[dev].store(true, std::memory_order_relaxed);
     return D2P_OK;
 }
-
-// Every argument of an attention call that the host can see.
-int check_attention(const d2p_attention_params* p);
-int check_strides(const d2p_strides& s, int rows, int heads, int D, int dtype, const char* name);
 
 }  // namespace enc
 }  // namespace d2p_amd
