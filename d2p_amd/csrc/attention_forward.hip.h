@@ -5,8 +5,8 @@
 // is the second operand of O^T = V^T P^T as it stands (encoder.hip.h).
 //
 // Bound, for 64 keys and 32 queries of 128 features of 16 bits: 32 MFMAs of 32 cycles against
-// 64 exponentials (16 cycles a wave) and about 100 other vector operations (4 cycles) a lane,
-// near 1000 cycles each on a SIMD, and 32 KiB of LDS reads for the wave, which four SIMDs'
+// 32 exponentials (16 cycles a wave) and about 150 other vector operations (4 cycles) a lane,
+// 1000 to 1100 cycles each on a SIMD, and 32 KiB of LDS reads for the wave, which four SIMDs'
 // matrix cores would take in those 1000 cycles too.  Two waves a SIMD, one's exponentials
 // beside the other's products; accumulators in architectural registers (256 a wave), where
 // the vector units read them without a copy.

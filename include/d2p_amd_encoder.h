@@ -38,7 +38,7 @@ typedef struct {
  *   p_i  = softmax of s_i over j (causal: over j <= at_i); zeros if there is no such j
  *   o_i  = sum_j p_ij d_ij v_j,  d_ij = 0 or 256 / (256 - drop)
  * Rows i >= nq of the result and of every gradient are zero.  Nothing at or past nq or nk
- * is used, whatever it holds.
+ * is used, whatever it holds, nor the bias of a distance that only such rows have.
  * Dropout: byte j % 4 of word i % 4 of Philox4x32 with 7 rounds (J. Salmon, M. Moraes,
  * R. Dror, D. Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011) on the counter
  * (j / 4, i / 4, b Hq + h, 0) and the key (low, high word of the seed) keeps the pair if it
