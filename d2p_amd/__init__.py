@@ -8,7 +8,8 @@ names) and the same ``torch.ops.d2p`` operator schemas, computed by hand-written
 kernels for CDNA4.  Tensors must live on the HIP device.
 
 Beside it stand the operators of the sequence encoders that make the scores' embeddings
-(``attention``, ``qk_norm_rope``, ``SequenceAttention``), which the reference does not have.
+(``attention``, ``qk_norm_rope``, ``SequenceAttention``; around them ``token_embedding``,
+``residual_norm``, ``SequenceEncoder``, ``clip_grad_norm_``), which the reference does not have.
 """
 from . import _ops
 from . import _compile  # noqa: F401  (fake/meta and autocast registrations)
@@ -18,6 +19,8 @@ from .dtw import soft_dtw, soft_dtw_sqeuclidean, DTWResult, SoftDTW
 from .nw import soft_nw, soft_nw_affine, NWResult, SoftNW, SoftNWAffine
 from .encoder import (attention, qk_norm_rope, relative_buckets, rope_tables, KeyValueCache,
                       SequenceAttention)
+from .stack import (token_embedding, residual_norm, global_norm, clip_gradients, clip_grad_norm_,
+                    SequenceEncoder)
 from . import ops
 
 # legacy flat names (reference d2p/__init__.py:120-139)
@@ -63,4 +66,6 @@ __all__ = [
     "soft_nw_affine_hvp", "soft_nw_affine_param_jacobian", "soft_nw_affine_backward_full",
     "attention", "qk_norm_rope", "relative_buckets", "rope_tables", "KeyValueCache",
     "SequenceAttention",
+    "token_embedding", "residual_norm", "global_norm", "clip_gradients", "clip_grad_norm_",
+    "SequenceEncoder",
 ]

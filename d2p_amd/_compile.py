@@ -134,6 +134,39 @@ _ENCODER_FAKES = {
         _contiguous(q), _contiguous(k),
         *(q.new_empty([q.size(3) if w else 0], dtype=torch.float32) for _ in range(2))),
 }
+
+
+def _typed(x, shape, dtype):
+    return x.new_empty(shape, dtype=dtype)
+
+
+def _residual(x, y, w, b, pw, pb, gate, norm, post, scale, rscale, eps, dtype, stats=False):
+    return (_contiguous(x) if y is not None else x.new_empty([0]),
+            _typed(x, x.shape, dtype) if norm else x.new_empty([0]),
+            _typed(x, [*x.shape[:2], 4] if stats else [0], torch.float32))
+
+
+def _residual_backward(dh, dn, h, y, stats, w, b, pw, pb, gate, norm, post, scale, rscale, eps,
+                       dtype, block, wanted):
+    same = not post and gate is None and scale == rscale and h.dtype == dtype
+    return (_contiguous(h), _typed(h, h.shape, dtype) if block and not same else h.new_empty([0]),
+            *(_contiguous(v) if v is not None and wanted >> i & 1 else h.new_empty([0])
+              for i, v in enumerate((gate, w, b, pw, pb))))
+
+
+_ENCODER_FAKES.update({
+    "token_embedding": lambda tokens, w, l, scale, padding, dtype: _typed(
+        w, [*tokens.shape, w.size(1)], dtype),
+    "token_embedding_backward": lambda grad, tokens, l, scale, padding, rows, dtype: _typed(
+        grad, [rows, grad.size(-1)], dtype),
+    "residual_norm": lambda *a: _residual(*a)[:2],
+    "residual_norm_forward": _residual,
+    "residual_norm_backward": _residual_backward,
+    "global_norm": lambda ts: _typed(ts[0], [], torch.float32),
+    "clip_gradients": lambda ts, m: ([torch.empty_like(t) for t in ts],
+                                     _typed(ts[0], [], torch.float32)),
+    "clip_gradients_into": lambda ts, m, out: _typed(ts[0], [], torch.float32),
+})
 for _name, _fn in _ENCODER_FAKES.items():
     register_fake(f"d2p_amd::{_name}")(_fn)
 

@@ -269,6 +269,21 @@ __device__ __forceinline__ float both_sum(float x) {
     return bits<float>(r.x) + bits<float>(r.y);
 }
 
+template <int CTRL> __device__ __forceinline__ float plus_dpp(float s) {
+    return s + bits<float>(__builtin_amdgcn_mov_dpp(bits<int>(s), CTRL, 0xf, 0xf, true));
+}
+// The sum over a group of lanes.  Neighbours by data-parallel moves: after the pairs and
+// the fours, mirroring eight lanes or sixteen brings the other half's sum.
+__device__ __forceinline__ float group_sum(float s, int lanes) {
+    if (lanes > 1) s = plus_dpp<0xB1>(s);
+    if (lanes > 2) s = plus_dpp<0x4E>(s);
+    if (lanes > 4) s = plus_dpp<0x141>(s);
+    if (lanes > 8) s = plus_dpp<0x140>(s);
+    if (lanes > 16) s += __shfl_xor(s, 16, 64);
+    if (lanes > 32) s = both_sum(s);
+    return s;
+}
+
 // Half precision has 5 bits of exponent.  What is rounded to it between two products is
 // scaled by powers of two, which change no bit of it in range and are undone in 32 bits:
 // probabilities by 2^FORWARD_SHIFT in the forward (at most 1 there) and 2^BACKWARD_SHIFT in

@@ -6,41 +6,14 @@
 // stream.  d2p_amd::attention and d2p_amd::qk_norm_rope differentiate; the operators that
 // do the work (attention_forward, attention_backward, qk_norm_rope_backward) go through
 // the dispatcher, so that fake tensors reach their fakes when a compiler traces.
-#include "torch_util.h"
+#include "encoder_util.h"
 
 #include <ATen/autocast_mode.h>
-#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 
 #include <cmath>
-#include <limits>
 #include <tuple>
 
-#include "../../include/d2p_amd_encoder.h"
-
 namespace {
-
-using torch::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::tensor_list;
-using OptTensor = c10::optional<Tensor>;
-
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-int type_code(const Tensor& t, const char* name) {
-    switch (t.scalar_type()) {
-        case torch::kFloat32: return D2P_FLOAT32;
-        case torch::kFloat16: return D2P_FLOAT16;
-        case torch::kBFloat16: return D2P_BFLOAT16;
-        default:
-            TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ",
-                        t.scalar_type());
-    }
-}
-
-int dim32(int64_t v, const char* what) {
-    TORCH_CHECK(v <= std::numeric_limits<int>::max(), what, " must fit int32, got ", v);
-    return (int)v;
-}
 
 void check_4d(const Tensor& t, const Tensor& like, const char* name) {
     TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
@@ -220,34 +193,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(
     return {dq, dk, dv, db};
 }
 
-template <class F> auto operator_handle(const char* name) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
-}
-
 auto call_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths,
                   bool causal, double scale, const OptTensor& bias, const OptTensor& buckets,
                   double dropout, int64_t seed, const OptTensor& seed_tensor) {
     static auto op = operator_handle<decltype(attention_forward)>("d2p_amd::attention_forward");
     return op.call(q, k, v, lengths, causal, scale, bias, buckets, dropout, seed, seed_tensor);
 }
-
-// A backward pass that nobody differentiates skips the autograd layer of the operators it
-// calls; in one that somebody does, that layer makes their derivative raise.
-struct BelowAutograd {
-    c10::optional<at::AutoDispatchBelowADInplaceOrView> guard;
-    BelowAutograd() {
-        if (!at::GradMode::is_enabled()) guard.emplace();
-    }
-};
-
-// Forward-mode derivatives are not implemented: a tangent raises, with and without gradients.
-void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
-    for (const Tensor* t : ts)
-        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name,
-                                    " does not support forward AD");
-}
-
-OptTensor saved(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
 class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
    public:
@@ -283,13 +234,6 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
                 Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-
-bool differentiates(std::initializer_list<const Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor* t : ts)
-        if (t->defined() && t->requires_grad()) return true;
-    return false;
-}
 
 Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& lengths,
                  bool causal, double scale, const OptTensor& bias, const OptTensor& buckets,

@@ -130,21 +130,6 @@ template <class T, int VEC> struct Lane {
     }
 };
 
-template <int CTRL> __device__ __forceinline__ float plus_dpp(float s) {
-    return s + bits<float>(__builtin_amdgcn_mov_dpp(bits<int>(s), CTRL, 0xf, 0xf, true));
-}
-// The sum over a group of lanes.  Neighbours by data-parallel moves: after the pairs and
-// the fours, mirroring eight lanes or sixteen brings the other half's sum.
-__device__ __forceinline__ float group_sum(float s, int lanes) {
-    if (lanes > 1) s = plus_dpp<0xB1>(s);
-    if (lanes > 2) s = plus_dpp<0x4E>(s);
-    if (lanes > 4) s = plus_dpp<0x141>(s);
-    if (lanes > 8) s = plus_dpp<0x140>(s);
-    if (lanes > 16) s += __shfl_xor(s, 16, 64);
-    if (lanes > 32) s = both_sum(s);
-    return s;
-}
-
 template <class T>
 __device__ __forceinline__ const T* row_of(const void* base, const d2p_strides& s, int b, int l,
                                            int h) {
