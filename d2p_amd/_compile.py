@@ -141,16 +141,16 @@ def _typed(x, shape, dtype):
 
 
 def _residual(x, y, w, b, pw, pb, gate, norm, post, scale, rscale, eps, dtype, stats=False):
-    return (_contiguous(x) if y is not None else x.new_empty([0]),
-            _typed(x, x.shape, dtype) if norm else x.new_empty([0]),
-            _typed(x, [*x.shape[:2], 4] if stats else [0], torch.float32))
+    return (_contiguous(x) if y is not None else None,
+            _typed(x, x.shape, dtype) if norm else None,
+            _typed(x, [*x.shape[:2], 4], torch.float32) if stats else None)
 
 
 def _residual_backward(dh, dn, h, y, stats, w, b, pw, pb, gate, norm, post, scale, rscale, eps,
                        dtype, block, wanted):
     same = not post and gate is None and scale == rscale and h.dtype == dtype
-    return (_contiguous(h), _typed(h, h.shape, dtype) if block and not same else h.new_empty([0]),
-            *(_contiguous(v) if v is not None and wanted >> i & 1 else h.new_empty([0])
+    return (_contiguous(h), _typed(h, h.shape, dtype) if block and not same else None,
+            *(_contiguous(v) if v is not None and wanted >> i & 1 else None
               for i, v in enumerate((gate, w, b, pw, pb))))
 
 

@@ -279,7 +279,11 @@ __device__ __forceinline__ float group_sum(float s, int lanes) {
     if (lanes > 2) s = plus_dpp<0x4E>(s);
     if (lanes > 4) s = plus_dpp<0x141>(s);
     if (lanes > 8) s = plus_dpp<0x140>(s);
-    if (lanes > 16) s += __shfl_xor(s, 16, 64);
+    if (lanes > 16) {   // rows of sixteen lanes, two and two
+        const u2v r = bits<u2v>(__builtin_amdgcn_permlane16_swap(bits<unsigned>(s),
+                                                                 bits<unsigned>(s), false, false));
+        s = bits<float>(r.x) + bits<float>(r.y);
+    }
     if (lanes > 32) s = both_sum(s);
     return s;
 }

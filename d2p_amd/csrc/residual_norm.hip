@@ -20,6 +20,7 @@ struct ResidualArgs {
     void *h, *n;
     float* stats;
     int lanes;
+    Divisor by_length;
 };
 
 // The learned vectors of a call in LDS, in 32 bits: `lanes` runs each, zeros behind D.  (In
@@ -46,45 +47,71 @@ struct Vectors {
         for (int e = 0; e < 4; ++e) { x[e] = lo[e]; x[4 + e] = hi[e]; }
     }
 };
-// the forward pass keeps W, PW, PC and C, the backward pass FEATURE_GATE in C's place
-enum Vector { W, PW, PC, C, FEATURE_GATE = C, VECTORS };
+// the forward pass keeps W, PW, PC and C; the backward pass, in C's place, what of scale * gate all
+// rows have alike
+enum Vector { W, PW, PC, C, GATED = C, VECTORS };
 constexpr int SLOTS = 64;       // numbers of a Team's slots, at the start of the LDS
 
 // v's mean (none for D2P_NORM_RMS) and 1 / sqrt(its spread + eps)
 template <bool WIDE>
-__device__ __forceinline__ float2 norm_stats(Team<WIDE>& team, int kind, const float* v, int left,
-                                             int D, float eps) {
+__device__ __forceinline__ float2 norm_stats(Team<WIDE>& team, int kind, const float* v,
+                                             const float* there, int D, float eps) {
     float2 s = {0.0f, 0.0f};
     if (kind == D2P_NORM_LAYER) {
-        s = team.spread(v, left, D);
+        s = team.spread(v, there, D);
     } else {
         float q = 0.0f;
 #pragma unroll
         for (int e = 0; e < RUN; ++e) q += v[e] * v[e];
         s.y = team.sum(q);
     }
-    return {s.x, 1.0f / sqrtf(s.y / D + eps)};
+    return {s.x, inverse_root(divided(s.y, (float)D) + eps)};
 }
 
-template <class T>
-__device__ __forceinline__ const T* row_at(const void* base, const d2p_row_strides& s, int b,
-                                           int l) {
-    return (const T*)base + b * s.batch + l * s.row;
-}
+// Where a row begins, and a lane's run in it.
+struct Place {
+    const d2p_residual_norm_params& p;
+    unsigned b, l;
+    int at;
+    long long flat;     // the row in a contiguous tensor
+
+    __device__ __forceinline__ Place(const d2p_residual_norm_params& p_, const Divisor& by_length,
+                                     unsigned row, int at_)
+        : p(p_), at(at_), flat((long long)row * p_.D) {
+        b = by_length(row);
+        l = row - b * p.L;
+    }
+    // (the strides of a contiguous tensor are told apart once for all lanes)
+    template <class T>
+    __device__ __forceinline__ const T* in(const void* base, const d2p_row_strides& s) const {
+        const bool dense = s.row == p.D && s.batch == (long long)p.L * p.D;
+        return (const T*)base + (dense ? flat : (long long)b * s.batch + (long long)l * s.row);
+    }
+};
 
 // a gate by sequence or token, in float32 or the block's type
-template <class TY>
-__device__ __forceinline__ void load_gate(const d2p_residual_norm_params& p, int b, int l, int at,
-                                          int have, float* gate) {
-    if (p.gate_dtype == p.block_dtype)
-        load_run(row_at<TY>(p.gate, p.gate_strides, b, l) + at, have, gate);
-    else
-        load_run(row_at<float>(p.gate, p.gate_strides, b, l) + at, have, gate);
-}
+template <class TY, bool EVEN> struct GateRun {
+    Eight<float> wide;
+    Eight<TY> narrow;
 
-// TX: the stream's type; TY: the block's
-// MOST: threads of a workgroup at most
-template <class TX, class TY, bool BLOCK, int MOST>
+    __device__ __forceinline__ void load(const Place& place) {
+        const d2p_residual_norm_params& p = place.p;
+        if (sizeof(TY) == 4 || p.gate_dtype == D2P_FLOAT32)
+            wide = load_run(place.in<float>(p.gate, p.gate_strides), place.at, p.D);
+        else
+            narrow = load_run(place.in<TY>(p.gate, p.gate_strides), place.at, p.D);
+    }
+    __device__ __forceinline__ void get(const Place& place, bool wanted, float* x) const {
+        const d2p_residual_norm_params& p = place.p;
+        if (sizeof(TY) == 4 || p.gate_dtype == D2P_FLOAT32)
+            unpack<EVEN>(wide, place.at, p.D, wanted, x);
+        else
+            unpack<EVEN>(narrow, place.at, p.D, wanted, x);
+    }
+};
+
+// EVEN: rows of whole runs; MOST: threads of a workgroup at most
+template <class TX, class TY, bool BLOCK, bool EVEN, int MOST>
 __global__ void __launch_bounds__(MOST) residual_norm_kernel(ResidualArgs a) {
     constexpr bool WIDE = MOST > 256;
     extern __shared__ __align__(16) float lds[];
@@ -108,40 +135,53 @@ __global__ void __launch_bounds__(MOST) residual_norm_kernel(ResidualArgs a) {
         vec.scale(PC, gate, p.scale, D);
     }
     __syncthreads();
-    // (all teams of a workgroup take as many turns: they meet in their sums)
+    float there[RUN];
+#pragma unroll
+    for (int e = 0; e < RUN; ++e) there[e] = e < left ? 1.0f : 0.0f;
+    // (all teams of a workgroup take as many turns: they meet in their sums.  Behind a row's end
+    // all is zero: what is loaded, and the vectors that it is multiplied with)
     for (unsigned base = blockIdx.x * teams; base < rows; base += gridDim.x * teams) {
         const unsigned row = base + threadIdx.x / a.lanes;
         const int have = row < rows ? left : 0;
-        const int b = row / (unsigned)p.L, l = row % (unsigned)p.L;
+        // (a team that is left over reads the last row again)
+        const Place place(p, a.by_length, min(row, rows - 1), at);
+        const int vat = fresh(at, base);    // the vectors are read anew, not kept in registers
         float v[RUN], x[RUN], w[RUN], c[RUN];
         float2 s = {0.0f, 0.0f}, ps = {0.0f, 0.0f};
-        load_run(row_at<TX>(a.x, p.x, b, l) + at, have, x);
+        const Eight<TX> rx = load_run(place.in<TX>(a.x, p.x), at, D);
+        Eight<TY> ry;
+        GateRun<TY, EVEN> rg;
         if (BLOCK) {
-            load_run(row_at<TY>(a.y, p.y, b, l) + at, have, v);
-            if (by_row) load_gate<TY>(p, b, l, at, have, c);
+            ry = load_run(place.in<TY>(a.y, p.y), at, D);
+            if (by_row) rg.load(place);
+        }
+        unpack<EVEN>(rx, at, D, true, x);
+        if (BLOCK) {
+            unpack<EVEN>(ry, at, D, true, v);
+            if (by_row) rg.get(place, true, c);
             if (p.post_norm != D2P_NORM_NONE) {
-                ps = norm_stats(team, p.post_norm, v, left, D, p.eps);
+                ps = norm_stats(team, p.post_norm, v, there, D, p.eps);
 #pragma unroll
                 for (int e = 0; e < RUN; ++e) v[e] = (v[e] - ps.x) * ps.y;
             }
             float pw[RUN], pc[RUN];
-            vec.get(PW, at, pw);
-            vec.get(PC, at, pc);
+            vec.get(PW, vat, pw);
+            vec.get(PC, vat, pc);
 #pragma unroll
             for (int e = 0; e < RUN; ++e) {
                 v[e] = v[e] * pw[e] + pc[e];
                 if (by_row) v[e] *= c[e];
-                x[e] = e < left ? p.residual_scale * x[e] + v[e] : 0.0f;
+                x[e] = p.residual_scale * x[e] + v[e];
             }
-            store_run((TX*)a.h + (long long)row * D + at, have, x);
+            store_run((TX*)a.h + place.flat + at, have, x);
         }
         if (p.norm != D2P_NORM_NONE) {
-            s = norm_stats(team, p.norm, x, left, D, p.eps);
-            vec.get(W, at, w);
-            vec.get(C, at, c);
+            s = norm_stats(team, p.norm, x, there, D, p.eps);
+            vec.get(W, vat, w);
+            vec.get(C, vat, c);
 #pragma unroll
             for (int e = 0; e < RUN; ++e) v[e] = (x[e] - s.x) * s.y * w[e] + c[e];
-            store_run((TY*)a.n + (long long)row * D + at, have, v);
+            store_run((TY*)a.n + place.flat + at, have, v);
         }
         if (a.stats && team.n == 0 && row < rows)
             *(f4v*)(a.stats + 4 * (long long)row) = f4v{s.x, s.y, ps.x, ps.y};
@@ -155,11 +195,14 @@ enum Sum { WEIGHT, BIAS, POST_WEIGHT, POST_BIAS, GATE, SUMS };
 
 struct ResidualBackArgs {
     d2p_residual_norm_params p;
-    const void *dh, *dn, *h, *y;
+    const void *dh, *dn, *stream, *y;   // stream: h for float32, x for 16 bits or without y
     const float* stats;
+    bool has_dh, has_dn, has_y;         // elsewise the pointer is to something else, of no stride
+    long long stats_step;               // 4, or 0 without stats
     void *dx, *dy, *dgate;
     float* partial[SUMS];   // [workgroups][D]; the gate's: [segments][D]; null: not wanted
     int lanes;
+    Divisor by_length;
     int batches, length;    // rows as segments are cut from them: [B, L], or [1, B L]
     int splits;             // segments of `length` rows
 };
@@ -182,9 +225,12 @@ __device__ __forceinline__ void flush(float* lds, const float* sums, float* dst,
     }
 }
 
-template <class TX, class TY, bool BLOCK, int MOST>
-__global__ void __launch_bounds__(MOST) residual_norm_backward_kernel(ResidualBackArgs a) {
-    constexpr bool WIDE = MOST > 256;
+// BLOCK: y has a gradient of its own (or, in 16 bits, h is formed from it again); BIASES: some
+// bias wants its gradient
+template <class TX, class TY, bool BLOCK, bool BIASES, bool EVEN, int MOST>
+__global__ void __launch_bounds__(MOST, BIASES && MOST == 256 ? 3 : 4)
+residual_norm_backward_kernel(ResidualBackArgs a) {
+    constexpr bool WIDE = MOST > 256, AGAIN = BLOCK && sizeof(TX) == 2;
     // the teams' slots; the vectors; then, for the teams' sums, eight numbers a thread
     extern __shared__ __align__(16) float lds[];
     const d2p_residual_norm_params& p = a.p;
@@ -193,13 +239,15 @@ __global__ void __launch_bounds__(MOST) residual_norm_backward_kernel(ResidualBa
     const int teams = blockDim.x / a.lanes;
     Vectors vec(lds + SLOTS, a.lanes);
     const bool by_row = p.gate_kind > D2P_GATE_FEATURE, post = p.post_norm != D2P_NORM_NONE;
-    if (a.dn) vec.load(W, p.weight, 1.0f, D);
+    if (a.has_dn) vec.load(W, p.weight, 1.0f, D);
     if (BLOCK) {
         vec.load(PW, p.post_weight, 1.0f, D);
         vec.load(PC, p.post_bias, 0.0f, D);
-        if (!by_row) vec.load(FEATURE_GATE, {p.gate, p.gate_dtype}, 1.0f, D);
+        vec.load(GATED, {by_row ? nullptr : p.gate, p.gate_dtype}, 1.0f, D);
+        vec.scale(GATED, {}, p.scale, D);
     }
     __syncthreads();
+    // Behind a row's end H is no zero after n's norm, but then meets vectors that are.
     float sums[SUMS][RUN] = {};
     const int segments = a.batches * a.splits;
     for (int seg = blockIdx.x; seg < segments; seg += gridDim.x) {
@@ -210,96 +258,132 @@ __global__ void __launch_bounds__(MOST) residual_norm_backward_kernel(ResidualBa
         for (unsigned base = r0; base < r1; base += teams) {
             const unsigned row = base + threadIdx.x / a.lanes;
             const int have = row < r1 ? left : 0;
-            const int b = row / (unsigned)p.L, l = row % (unsigned)p.L;
-            const long long flat = (long long)row * D + at;
-            float H[RUN], dn[RUN], hh[RUN], y[RUN], gate[RUN], w[RUN];
-            f4v st = {};
-            if (a.stats && row < r1) st = *(const f4v*)(a.stats + 4 * (long long)row);
-            load_run(row_at<TX>(a.dh, p.dh, b, l) + at, a.dh ? have : 0, H);
-            if (a.dn) {
-                load_run(row_at<TY>(a.dn, p.dn, b, l) + at, have, dn);
-                load_run(row_at<TX>(a.h, p.x, b, l) + at, have, hh);
-            }
+            // (a team that is left over reads the last row again, and adds zeros)
+            // (what a lane's place in the row gives is computed in each turn: kept, it would
+            // take more registers than there are)
+            const int vat = fresh(at, base);
+            const Place place(p, a.by_length, min(row, r1 - 1), vat);
+            const long long flat = place.flat + vat;
+            float H[RUN], dn[RUN], hh[RUN], y[RUN], gate[RUN], w[RUN], c[RUN];
+            // (what is not there is read all the same, from one row of something else that is, and
+            // taken for zeros: no load waits for a branch)
+            Eight<TY> ry;
+            GateRun<TY, EVEN> rg;
+            f4v st = *(const f4v*)(a.stats + a.stats_step * min(row, r1 - 1));
+            const Eight<TX> rdh = load_run(place.in<TX>(a.dh, p.dh), vat, D);
+            const Eight<TY> rdn = load_run(place.in<TY>(a.dn, p.dn), vat, D);
+            const Eight<TX> rs = load_run(place.in<TX>(a.stream, p.x), vat, D);
             if (BLOCK) {
-                load_run(row_at<TY>(a.y, p.y, b, l) + at, a.y ? have : 0, y);
-                if (by_row) load_gate<TY>(p, b, l, at, have, gate);
+                ry = load_run(place.in<TY>(a.y, p.y), vat, D);
+                if (by_row) rg.load(place);
             }
-            if (a.dn) {
+            const bool there = row < r1;
+            if (BLOCK) {
+                // without a norm of its own z is y: mean 0, one over the spread 1, weight 1, bias 0
+                st[2] = post ? st[2] : 0.0f;
+                st[3] = post ? st[3] : 1.0f;
+                unpack<EVEN>(ry, vat, D, there && a.has_y, y);
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) y[e] = (y[e] - st[2]) * st[3];
+            }
+            if (a.has_dn) {
+                unpack<EVEN>(rs, vat, D, there, hh);
+                if (AGAIN) {
+                    vec.get(PW, vat, w);
+                    vec.get(PC, vat, c);
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e) w[e] = y[e] * w[e] + c[e];
+                    vec.get(GATED, vat, c);
+                    if (by_row) {
+                        rg.get(place, there, gate);
+#pragma unroll
+                        for (int e = 0; e < RUN; ++e) c[e] *= gate[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < RUN; ++e) hh[e] = p.residual_scale * hh[e] + c[e] * w[e];
+                }
                 float2 m = {0.0f, 0.0f};
-                vec.get(W, at, w);
+                vec.get(W, vat, w);
+                unpack<EVEN>(rdn, vat, D, there, dn);
 #pragma unroll
                 for (int e = 0; e < RUN; ++e) {
                     hh[e] = (hh[e] - st[0]) * st[1];
                     sums[WEIGHT][e] += dn[e] * hh[e];
-                    sums[BIAS][e] += dn[e];
+                    if (BIASES) sums[BIAS][e] += dn[e];
                     dn[e] *= w[e];
                     m.x += dn[e];
                     m.y += dn[e] * hh[e];
                 }
                 if (p.norm == D2P_NORM_LAYER) m = team.sum(m.x, m.y);
                 else m = {0.0f, team.sum(m.y)};
-                m.x /= D;
-                m.y /= D;
+                m.x = divided(m.x, (float)D);
+                m.y = divided(m.y, (float)D);
+                unpack<EVEN>(rdh, vat, D, there && a.has_dh, H);
 #pragma unroll
-                for (int e = 0; e < RUN; ++e)
-                    H[e] = e < have ? H[e] + st[1] * (dn[e] - m.x - hh[e] * m.y) : 0.0f;
+                for (int e = 0; e < RUN; ++e) H[e] += st[1] * (dn[e] - m.x - hh[e] * m.y);
+            } else {
+                unpack<EVEN>(rdh, vat, D, there && a.has_dh, H);
             }
-            float dx[RUN];
 #pragma unroll
-            for (int e = 0; e < RUN; ++e) dx[e] = p.residual_scale * H[e];
-            store_run((TX*)a.dx + flat, have, dx);
-            if (!BLOCK) continue;       // no y, or its gradient is x's
-            float2 m = {0.0f, 0.0f};
-            float dgate[RUN], pc[RUN];
-            if (!by_row) vec.get(FEATURE_GATE, at, gate);
+            for (int e = 0; e < RUN; ++e) c[e] = p.residual_scale * H[e];
+            store_run((TX*)a.dx + flat, have, c);
+            if (!BLOCK || !a.dy) continue;      // no y, or its gradient is x's
+            if (a.dgate) {
+                vec.get(PW, vat, w);
+                vec.get(PC, vat, c);
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) {
+                    c[e] = p.scale * H[e] * (y[e] * w[e] + c[e]);
+                    sums[GATE][e] += c[e];
+                }
+                if (p.gate_kind == D2P_GATE_TOKEN) {
+                    if (p.gate_dtype == D2P_FLOAT32) store_run((float*)a.dgate + flat, have, c);
+                    else store_run((TY*)a.dgate + flat, have, c);
+                }
+            }
+            vec.get(GATED, vat, c);
+            if (by_row) {
+                rg.get(place, there, gate);
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) c[e] *= gate[e];
+            }
+#pragma unroll
+            for (int e = 0; e < RUN; ++e) H[e] *= c[e];
             if (post) {
-                vec.get(PW, at, w);
-                vec.get(PC, at, pc);
-            }
+                float2 m = {0.0f, 0.0f};
+                vec.get(PW, vat, w);
 #pragma unroll
-            for (int e = 0; e < RUN; ++e) {
-                if (post) y[e] = e < have ? (y[e] - st[2]) * st[3] : 0.0f;
-                H[e] *= p.scale;
-                dgate[e] = H[e] * (post ? y[e] * w[e] + pc[e] : y[e]);
-                sums[GATE][e] += dgate[e];
-                H[e] *= gate[e];
-                if (post) {
+                for (int e = 0; e < RUN; ++e) {
                     sums[POST_WEIGHT][e] += H[e] * y[e];
-                    sums[POST_BIAS][e] += H[e];
+                    if (BIASES) sums[POST_BIAS][e] += H[e];
                     H[e] *= w[e];
                     m.x += H[e];
                     m.y += H[e] * y[e];
                 }
-            }
-            if (a.dgate && p.gate_kind == D2P_GATE_TOKEN) {
-                if (p.gate_dtype == p.block_dtype) store_run((TY*)a.dgate + flat, have, dgate);
-                else store_run((float*)a.dgate + flat, have, dgate);
-            }
-            if (post) {
                 if (p.post_norm == D2P_NORM_LAYER) m = team.sum(m.x, m.y);
                 else m = {0.0f, team.sum(m.y)};
-                m.x /= D;
-                m.y /= D;
+                m.x = divided(m.x, (float)D);
+                m.y = divided(m.y, (float)D);
 #pragma unroll
                 for (int e = 0; e < RUN; ++e) H[e] = st[3] * (H[e] - m.x - y[e] * m.y);
             }
             store_run((TY*)a.dy + flat, have, H);
         }
         if (BLOCK && a.partial[GATE]) {
-            flush(lds + SLOTS + VECTORS * vec.padded, sums[GATE], a.partial[GATE] + (long long)seg * D, a.lanes, D);
+            flush(lds + SLOTS + VECTORS * vec.padded, sums[GATE],
+                  a.partial[GATE] + (long long)seg * D, a.lanes, D);
 #pragma unroll
             for (int e = 0; e < RUN; ++e) sums[GATE][e] = 0.0f;
         }
     }
 #pragma unroll
     for (int k = 0; k < GATE; ++k)
-        if ((BLOCK || k < POST_WEIGHT) && a.partial[k])
-            flush(lds + SLOTS + VECTORS * vec.padded, sums[k], a.partial[k] + (long long)blockIdx.x * D, a.lanes, D);
+        if ((BLOCK || k < POST_WEIGHT) && (BIASES || (k != BIAS && k != POST_BIAS)) && a.partial[k])
+            flush(lds + SLOTS + VECTORS * vec.padded, sums[k],
+                  a.partial[k] + (long long)blockIdx.x * D, a.lanes, D);
 }
 
 namespace {
-
-constexpr int MOST_GROUPS = 1024;   // workgroups of the backward pass at most
 
 int check_vector(const d2p_vector& v) {
     D2P_REQUIRE(!v.data || known_type(v.dtype), "unknown element type of a learned vector");
@@ -312,7 +396,7 @@ int check(const d2p_residual_norm_params* p) {
                 "unknown element types, or a pair other than equal ones and 16 bits beside float32");
     D2P_REQUIRE(p->B >= 0 && p->L >= 0, "negative size");
     D2P_REQUIRE((long long)p->B * p->L < 1LL << 31, "too many rows");
-    D2P_REQUIRE(p->D >= 1 && p->D <= 8192, "features must be between 1 and 8192");
+    D2P_REQUIRE(p->D >= RUN && p->D <= 8192, "features must be between 8 and 8192");
     for (int kind : {p->norm, p->post_norm})
         D2P_REQUIRE(kind >= D2P_NORM_NONE && kind <= D2P_NORM_LAYER, "unknown norm");
     for (const d2p_vector* v : {&p->weight, &p->bias, &p->post_weight, &p->post_bias})
@@ -327,10 +411,14 @@ int check(const d2p_residual_norm_params* p) {
     return D2P_OK;
 }
 
-// Strides of a gate that has one number for several rows say nothing.
+// Strides over one of something say nothing: those of a contiguous tensor stand in their place.
+d2p_row_strides plain(const d2p_row_strides& s, const d2p_residual_norm_params& p) {
+    const long long row = p.L > 1 ? s.row : p.D;
+    return {p.B > 1 ? s.batch : p.L * row, row};
+}
 d2p_row_strides gate_steps(const d2p_residual_norm_params& p) {
-    return {p.gate_kind >= D2P_GATE_SEQUENCE ? p.gate_strides.batch : 0,
-            p.gate_kind == D2P_GATE_TOKEN ? p.gate_strides.row : 0};
+    if (p.gate_kind == D2P_GATE_TOKEN) return plain(p.gate_strides, p);
+    return {p.gate_kind == D2P_GATE_SEQUENCE ? p.gate_strides.batch : 0, 0};
 }
 
 int threads_of(int lanes) { return std::max(lanes, 256); }
@@ -347,29 +435,38 @@ int launch(const char* name, void (*kernel)(Args), LdsAllowed& known, const Args
     D2P_HIP(hipGetLastError());
     return D2P_OK;
 }
-template <class TX, class TY, bool BLOCK, int MOST>
+template <class TX, class TY, bool BLOCK, bool EVEN, int MOST>
 int launch_forward(const ResidualArgs& a, int grid, hipStream_t st) {
     static LdsAllowed known;
-    return launch("residual_norm", residual_norm_kernel<TX, TY, BLOCK, MOST>, known, a, grid, false,
-                  st);
+    return launch("residual_norm", residual_norm_kernel<TX, TY, BLOCK, EVEN, MOST>, known, a, grid,
+                  false, st);
 }
-template <class TX, class TY, bool BLOCK, int MOST>
+template <class TX, class TY, bool BLOCK, bool EVEN, int MOST>
 int launch_backward(const ResidualBackArgs& a, int grid, hipStream_t st) {
-    static LdsAllowed known;
-    return launch("residual_norm_backward", residual_norm_backward_kernel<TX, TY, BLOCK, MOST>,
-                  known, a, grid, true, st);
+    static LdsAllowed known[2];
+    if (a.partial[BIAS] || a.partial[POST_BIAS])
+        return launch("residual_norm_backward",
+                      residual_norm_backward_kernel<TX, TY, BLOCK, true, EVEN, MOST>, known[1], a,
+                      grid, true, st);
+    return launch("residual_norm_backward",
+                  residual_norm_backward_kernel<TX, TY, BLOCK, false, EVEN, MOST>, known[0], a, grid,
+                  true, st);
 }
 
-// f(threads of a workgroup at most): rows within a wave, or of waves that leave a thread 256
-// registers, or of more
-template <class F> int by_lanes(int lanes, F f) {
-    return lanes <= 64    ? f(std::integral_constant<int, 256>{})
-           : lanes <= 512 ? f(std::integral_constant<int, 512>{})
-                          : f(std::integral_constant<int, 1024>{});
+// f(rows of whole runs, threads of a workgroup at most): rows within a wave, or of several
+template <class F> int by_row(int D, F f) {
+    using std::integral_constant;
+    const bool even = D % RUN == 0;
+    if (D <= 64 * RUN)
+        return even ? f(std::true_type{}, integral_constant<int, 256>{})
+                    : f(std::false_type{}, integral_constant<int, 256>{});
+    return even ? f(std::true_type{}, integral_constant<int, 1024>{})
+                : f(std::false_type{}, integral_constant<int, 1024>{});
 }
 
-// How the backward pass cuts rows into segments: at most MOST_GROUPS of them, four turns of a
-// workgroup at least, and each of one sequence where the gate's gradient is by sequence.
+// How the backward pass cuts rows into segments: at most as many as the card's 256 compute units
+// hold at four waves a SIMD, no fewer while there are rows for it, and each of one sequence
+// where the gate's gradient is by sequence.
 struct Cut {
     int batches, length, splits, grid;
     Cut(const d2p_residual_norm_params& p, int lanes) {
@@ -377,9 +474,10 @@ struct Cut {
         const bool by_sequence = p.gate_kind == D2P_GATE_SEQUENCE;
         batches = by_sequence ? p.B : 1;
         length = by_sequence ? p.L : p.B * p.L;
-        const int most = std::max(1, MOST_GROUPS / std::max(batches, 1));
-        splits = std::min(most, std::max(1, length / (4 * teams)));
-        grid = (int)std::min<long long>((long long)batches * splits, MOST_GROUPS);
+        const int groups = 256 * 1024 / threads_of(lanes);
+        const int most = std::max(1, groups / std::max(batches, 1));
+        splits = std::min(most, std::max(1, cdiv(length, teams)));
+        grid = (int)std::min<long long>((long long)batches * splits, groups);
     }
 };
 
@@ -398,7 +496,8 @@ extern "C" int d2p_residual_norm(const d2p_residual_norm_params* p, const void* 
     D2P_REQUIRE(!y == !h && !y == !p->with_y, "with_y, y and h go together");
     D2P_REQUIRE(y || (p->post_norm == D2P_NORM_NONE && p->gate_kind == D2P_GATE_NONE),
                 "a gate or a second norm needs y");
-    ResidualArgs a{*p, x, y, h, n, stats, team_of(p->D)};
+    ResidualArgs a{*p, x, y, h, n, stats, team_of(p->D), Divisor(p->L)};
+    for (d2p_row_strides* s : {&a.p.x, &a.p.y}) *s = plain(*s, *p);
     a.p.gate_strides = gate_steps(*p);
     const int teams = threads_of(a.lanes) / a.lanes;
     const int most = 8 * 256 * std::max(device_cus(), 1) / threads_of(a.lanes);
@@ -407,17 +506,15 @@ extern "C" int d2p_residual_norm(const d2p_residual_norm_params* p, const void* 
         using TX = typename decltype(tx)::type;
         using TY = typename decltype(ty)::type;
         const auto st = (hipStream_t)stream;
-        return y ? by_lanes(a.lanes, [&](auto most) {
-                       return launch_forward<TX, TY, true, most()>(a, grid, st);
-                   })
-                 : by_lanes(a.lanes, [&](auto most) {
-                       return launch_forward<TX, TY, false, most()>(a, grid, st);
-                   });
+        return by_row(p->D, [&](auto even, auto most) {
+            return y ? launch_forward<TX, TY, true, even(), most()>(a, grid, st)
+                     : launch_forward<TX, TY, false, even(), most()>(a, grid, st);
+        });
     });
 }
 
 extern "C" size_t d2p_residual_norm_backward_workspace_bytes(const d2p_residual_norm_params* p) {
-    if (!p || p->B < 0 || p->L < 0 || p->D < 1 || p->D > 8192 || (long long)p->B * p->L >= 1LL << 31)
+    if (!p || p->B < 0 || p->L < 0 || p->D < RUN || p->D > 8192 || (long long)p->B * p->L >= 1LL << 31)
         return 0;
     const Cut cut(*p, team_of(p->D));
     const size_t gate = p->gate_kind == D2P_GATE_FEATURE || p->gate_kind == D2P_GATE_SEQUENCE
@@ -426,18 +523,20 @@ extern "C" size_t d2p_residual_norm_backward_workspace_bytes(const d2p_residual_
 }
 
 extern "C" int d2p_residual_norm_backward(const d2p_residual_norm_params* p, const void* dh,
-                                          const void* dn, const void* h, const void* y,
+                                          const void* dn, const void* stream_in, const void* y,
                                           const float* stats, void* dx, void* dy, void* dgate,
                                           void* dweight, void* dbias, void* dpost_weight,
                                           void* dpost_bias, void* workspace,
                                           size_t workspace_bytes, void* stream) {
     D2P_TRY(check(p));
-    const bool rows = (long long)p->B * p->L > 0;
+    const bool rows = (long long)p->B * p->L > 0, wide = p->dtype == D2P_FLOAT32;
     const bool norm = dn && p->norm != D2P_NORM_NONE;
+    const bool again = norm && p->with_y && !wide;      // h is formed anew
     if (rows) {
-        D2P_REQUIRE(dx && (!norm || (h && stats)), "null pointer argument");
+        D2P_REQUIRE(dh || norm, "dh or dn is needed");
+        D2P_REQUIRE(dx && (!norm || (stream_in && stats)), "null pointer argument");
         D2P_REQUIRE(p->post_norm == D2P_NORM_NONE || (y && stats), "null pointer argument");
-        D2P_REQUIRE(!dgate || y, "the gate's gradient needs y");
+        D2P_REQUIRE(y || !(dgate || again), "y is needed");
         D2P_REQUIRE(dy || (p->post_norm == D2P_NORM_NONE && p->gate_kind == D2P_GATE_NONE &&
                            (!p->with_y || (p->scale == p->residual_scale &&
                                            p->dtype == p->block_dtype))),
@@ -450,18 +549,29 @@ extern "C" int d2p_residual_norm_backward(const d2p_residual_norm_params* p, con
     ResidualBackArgs a{};
     a.p = *p;
     a.p.gate_strides = gate_steps(*p);
-    // h lies as the forward pass wrote it; without y it is x
-    if (p->with_y) a.p.x = {(long long)p->L * p->D, p->D};
-    else a.p.residual_scale = 1.0f;
-    a.dh = dh;
-    a.dn = norm ? dn : nullptr;
-    a.h = h;
-    a.y = y;
-    a.stats = stats;
+    if (p->with_y && wide) a.p.x = {(long long)p->L * p->D, p->D};
+    if (!p->with_y) a.p.residual_scale = 1.0f;
+    for (d2p_row_strides* s : {&a.p.x, &a.p.y, &a.p.dh, &a.p.dn}) *s = plain(*s, *p);
+    // dh and what n was formed from are of the wide type: a row of them has room for any
+    const void* const other = dh ? dh : stream_in;
+    auto or_else = [&](const void* x, d2p_row_strides& s) {
+        if (!x) s = {0, 0};
+        return x ? x : other;
+    };
+    a.has_dh = dh;
+    a.has_dn = norm;
+    a.has_y = y;
+    a.dh = or_else(dh, a.p.dh);
+    a.dn = or_else(norm ? dn : nullptr, a.p.dn);
+    a.stream = or_else(norm ? stream_in : nullptr, a.p.x);
+    a.y = or_else(y, a.p.y);
+    a.stats = stats ? stats : (const float*)other;
+    a.stats_step = stats ? 4 : 0;
     a.dx = dx;
     a.dy = dy;
     a.dgate = dgate;
     a.lanes = team_of(p->D);
+    a.by_length = Divisor(p->L);
     const Cut cut(*p, a.lanes);
     a.batches = cut.batches;
     a.length = cut.length;
@@ -487,12 +597,10 @@ extern "C" int d2p_residual_norm_backward(const d2p_residual_norm_params* p, con
             using TX = typename decltype(tx)::type;
             using TY = typename decltype(ty)::type;
             const auto st = (hipStream_t)stream;
-            return dy ? by_lanes(a.lanes, [&](auto most) {
-                            return launch_backward<TX, TY, true, most()>(a, cut.grid, st);
-                        })
-                      : by_lanes(a.lanes, [&](auto most) {
-                            return launch_backward<TX, TY, false, most()>(a, cut.grid, st);
-                        });
+            return by_row(p->D, [&](auto even, auto most) {
+                return dy || again ? launch_backward<TX, TY, true, even(), most()>(a, cut.grid, st)
+                                   : launch_backward<TX, TY, false, even(), most()>(a, cut.grid, st);
+            });
         }));
     return launch_sum_rows("residual_norm_vector_grads", jobs, (hipStream_t)stream);
 }

@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(SumJobs a) {
     s = 0.0f;
 #pragma unroll
     for (int w = 0; w < 16; ++w) s += part[w][lane];
-    store_as(job.dst, job.dtype, (long long)group * a.D + d, s);
+    store_as(job.dst, job.dtype, (long long)group * a.D + d, s * a.scale);
 }
 
 int launch_sum_rows(const char* name, const SumJobs& a, hipStream_t st) {

@@ -4,7 +4,7 @@
 // Forward: bound by writing the result; a team of lanes copies rows, eight numbers a lane.
 //
 // Backward: the gradient's rows of one token have to come together.  Positions are sorted by
-// token (a stable radix sort of 8 bits a pass, so that sums have one order), cut into chunks
+// token (a stable radix sort of up to ten bits a pass, so that sums have one order), cut into chunks
 // of equal length, and a team of lanes adds up its chunk's rows, run by run.  A run inside a
 // chunk goes to the table; one that crosses a border leaves its part in the workspace, and a
 // last kernel joins those.  Tokens that do not occur are marked by the sort's last pass, and
@@ -23,14 +23,17 @@ struct EmbedArgs {
     const void* weight;
     void* out;
     int lanes;
+    Divisor by_length;
 };
+constexpr int DEEP = 4;             // rows that a team has in flight
 
 // The token at position n of [B, L]: its row; ABSENT for padding and past its sequence's
 // length; WRONG for one that the table does not have or whose sequence's length is out of range.
 constexpr int ABSENT = -1, WRONG = -2;
-__device__ __forceinline__ int token_at(const d2p_token_embedding_params& p, int n) {
+__device__ __forceinline__ int token_at(const d2p_token_embedding_params& p,
+                                        const Divisor& by_length, int n) {
     if (p.lengths) {
-        const int l = n % p.L, length = p.lengths[n / p.L];
+        const int b = by_length(n), l = n - b * p.L, length = p.lengths[b];
         if (length < 0 || length > p.L) return WRONG;
         if (l >= length) return ABSENT;
     }
@@ -44,16 +47,27 @@ template <class TW, class TO>
 __global__ void __launch_bounds__(256) token_embedding_kernel(EmbedArgs a) {
     const d2p_token_embedding_params& p = a.p;
     const int n0 = threadIdx.x & (a.lanes - 1), teams = 256 / a.lanes;
-    const int rows = p.B * p.L;
+    const long long rows = (long long)p.B * p.L, step = (long long)gridDim.x * teams;
     for (long long row = (long long)blockIdx.x * teams + threadIdx.x / a.lanes; row < rows;
-         row += (long long)gridDim.x * teams) {
-        const int t = token_at(p, (int)row);
-        for (int at = n0 * RUN; at < p.D; at += a.lanes * RUN) {
-            float x[RUN];
-            load_run((const TW*)a.weight + (long long)max(t, 0) * p.D + at, t < 0 ? 0 : p.D - at, x);
+         row += DEEP * step) {
+        int t[DEEP];
 #pragma unroll
-            for (int e = 0; e < RUN; ++e) x[e] = t == WRONG ? __builtin_nanf("") : x[e] * p.scale;
-            store_run((TO*)a.out + row * p.D + at, p.D - at, x);
+        for (int u = 0; u < DEEP; ++u)
+            t[u] = row + u * step < rows ? token_at(p, a.by_length, (int)(row + u * step)) : ABSENT;
+        for (int at = n0 * RUN; at < p.D; at += a.lanes * RUN) {
+            Eight<TW> r[DEEP];
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u)
+                r[u] = load_run((const TW*)a.weight + (long long)max(t[u], 0) * p.D, at, p.D);
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u) {
+                float x[RUN];
+                unpack(r[u], at, p.D, t[u] >= 0, x);
+#pragma unroll
+                for (int e = 0; e < RUN; ++e) x[e] = t[u] == WRONG ? __builtin_nanf("") : x[e] * p.scale;
+                if (row + u * step < rows)
+                    store_run((TO*)a.out + (row + u * step) * p.D + at, p.D - at, x);
+            }
         }
     }
 }
@@ -61,23 +75,25 @@ __global__ void __launch_bounds__(256) token_embedding_kernel(EmbedArgs a) {
 // ---------------------------------------------------------------------------
 // sort
 // ---------------------------------------------------------------------------
-constexpr int DIGITS = 256, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
-constexpr int MOST_TILES = 256;
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+constexpr int MOST_BITS = 10, MOST_TILES = 128;
 
 struct SortArgs {
     d2p_token_embedding_params p;
+    Divisor by_length;
     int N;                          // positions
-    int tiles, tile;                // of `tile` positions each
-    int shift, first, last;         // first, last pass
+    int tiles, tile_bits;           // of 1 << tile_bits positions each
+    int shift, bits;                // the digit of this pass
+    int first, last;                // first, last pass
     const unsigned *keys, *at;      // of the pass before: tokens (V for none) and positions
     unsigned *keys_to, *at_to;
-    unsigned* counts;               // [tiles][DIGITS]
+    unsigned* counts;               // [tiles][1 << bits]
     unsigned char* present;         // [V rounded up to 16]
 };
 
 __device__ __forceinline__ unsigned key_at(const SortArgs& a, int n) {
     if (!a.first) return a.keys[n];
-    const int t = token_at(a.p, n);
+    const int t = token_at(a.p, a.by_length, n);
     return t < 0 ? (unsigned)a.p.V : (unsigned)t;
 }
 
@@ -88,72 +104,85 @@ __device__ __forceinline__ void clear_present(const SortArgs& a, long long from,
 
 // How often each digit occurs in each tile; the first pass clears the marks too.
 __global__ void __launch_bounds__(SORT_THREADS) count_digits_kernel(SortArgs a) {
-    __shared__ unsigned count[DIGITS];
-    if (a.first)
-        clear_present(a, (long long)blockIdx.x * SORT_THREADS + threadIdx.x,
-                      (long long)gridDim.x * SORT_THREADS);
+    __shared__ unsigned count[1 << MOST_BITS];
+    const long long me = (long long)blockIdx.x * SORT_THREADS + threadIdx.x;
+    const long long all = (long long)gridDim.x * SORT_THREADS;
+    const int digits = 1 << a.bits;
+    if (a.first) clear_present(a, me, all);
     if ((int)blockIdx.x >= a.tiles) return;
-    if (threadIdx.x < DIGITS) count[threadIdx.x] = 0;
+    if ((int)threadIdx.x < digits) count[threadIdx.x] = 0;
     __syncthreads();
-    const long long n0 = (long long)blockIdx.x * a.tile;
-    const long long n1 = min(n0 + a.tile, (long long)a.N);
+    const long long n0 = (long long)blockIdx.x << a.tile_bits;
+    const long long n1 = min(n0 + (1LL << a.tile_bits), (long long)a.N);
     for (long long n = n0 + threadIdx.x; n < n1; n += SORT_THREADS)
-        atomicAdd(&count[key_at(a, (int)n) >> a.shift & (DIGITS - 1)], 1u);
+        atomicAdd(&count[key_at(a, (int)n) >> a.shift & (digits - 1)], 1u);
     __syncthreads();
-    if (threadIdx.x < DIGITS)
-        a.counts[(long long)blockIdx.x * DIGITS + threadIdx.x] = count[threadIdx.x];
+    if ((int)threadIdx.x < digits)
+        a.counts[(long long)blockIdx.x * digits + threadIdx.x] = count[threadIdx.x];
 }
 
+// What a sort keeps in LDS for digits of `bits` bits.
 struct SortLds {
-    unsigned wave[SORT_WAVES][DIGITS];   // of each wave's share: counts, then next places
-    unsigned base[DIGITS];
-    unsigned part[2][4][DIGITS];
-    unsigned scan[4];
-};
-
-// s.base[d] = keys of smaller digits anywhere + keys of digit d in the tiles before this one
-__device__ __forceinline__ void digit_bases(SortLds& s, const unsigned* counts, int tiles, int tile) {
-    const int d = threadIdx.x & (DIGITS - 1), g = threadIdx.x / DIGITS;
-    unsigned all = 0, before = 0;
-#pragma unroll 8
-    for (int t = g; t < tiles; t += 4) {
-        const unsigned c = counts[(long long)t * DIGITS + d];
-        all += c;
-        before += t < tile ? c : 0;
+    unsigned* wave;     // [SORT_WAVES][digits]: of each wave's share: counts, then next places
+    unsigned* base;     // [digits]: the next key's place
+    unsigned* part;     // [2][SORT_THREADS]
+    unsigned* scan;     // [SORT_WAVES]
+    int digits;
+    __device__ __forceinline__ SortLds(unsigned* lds, int bits) : digits(1 << bits) {
+        part = lds;
+        scan = part + 2 * SORT_THREADS;
+        base = scan + SORT_WAVES;
+        wave = base + digits;
     }
-    s.part[0][g][d] = all;
-    s.part[1][g][d] = before;
-    __syncthreads();
-    if (g == 0) {
-        all = before = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            all += s.part[0][i][d];
-            before += s.part[1][i][d];
-        }
+    static size_t bytes(int bits) {
+        return (2 * SORT_THREADS + SORT_WAVES + (size_t)(SORT_WAVES + 1) * (1 << bits)) * 4;
+    }
+    // base[d] = the `all` of smaller digits + before, by the thread of digit d (others: zeros)
+    __device__ __forceinline__ void set_bases(unsigned all, unsigned before) {
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
         unsigned sum = all;
-        const int lane = d & 63;
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             const unsigned x = __shfl_up(sum, o, 64);
             if (lane >= o) sum += x;
         }
-        if (lane == 63) s.scan[d >> 6] = sum;
-        s.base[d] = sum - all + before;
-    }
-    __syncthreads();
-    if (g == 0) {
+        if (lane == 63) scan[w] = sum;
+        __syncthreads();
+        if ((int)threadIdx.x >= digits) return;
         unsigned below = 0;
-        for (int w = 0; w < d >> 6; ++w) below += s.scan[w];
-        s.base[d] += below;
+        for (int i = 0; i < w; ++i) below += scan[i];
+        base[threadIdx.x] = below + sum - all + before;
     }
+};
+
+// The bases of a tile's digits: keys of smaller digits anywhere, keys of the digit in the tiles
+// before.  The threads that no digit has take a share of the tiles.
+__device__ __forceinline__ void digit_bases(SortLds& s, const unsigned* counts, int tiles, int tile) {
+    const int d = threadIdx.x & (s.digits - 1), g = threadIdx.x / s.digits;
+    const int groups = SORT_THREADS / s.digits;
+    unsigned all = 0, before = 0;
+#pragma unroll 16
+    for (int t = g; t < tiles; t += groups) {
+        const unsigned c = counts[(long long)t * s.digits + d];
+        all += c;
+        before += t < tile ? c : 0;
+    }
+    s.part[threadIdx.x] = all;
+    s.part[SORT_THREADS + threadIdx.x] = before;
+    __syncthreads();
+    all = before = 0;
+    if (g == 0)
+        for (int i = 0; i < groups; ++i) {
+            all += s.part[i * s.digits + d];
+            before += s.part[SORT_THREADS + i * s.digits + d];
+        }
+    s.set_bases(all, before);
 }
 
 // Lanes of the wave whose digit is this lane's, among the lanes that are `on`.
-__device__ __forceinline__ unsigned long long same_digit(unsigned digit, bool on) {
+__device__ __forceinline__ unsigned long long same_digit(unsigned digit, int bits, bool on) {
     unsigned long long m = __ballot(on);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
+    for (int b = 0; b < bits; ++b) {
         const unsigned long long ones = __ballot(digit >> b & 1);
         m &= digit >> b & 1 ? ones : ~ones;
     }
@@ -163,22 +192,24 @@ __device__ __forceinline__ unsigned long long same_digit(unsigned digit, bool on
 // One part of a tile of ITEMS keys a thread: wave w has the keys 64 ITEMS w .. of it, in order.
 // place[i]: where key i goes; s.base moves on by the part's counts.
 template <int ITEMS>
-__device__ __forceinline__ void place_keys(SortLds& s, const unsigned (&digit)[ITEMS], int here,
-                                           unsigned (&place)[ITEMS]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < SORT_WAVES * DIGITS; i += SORT_THREADS) (&s.wave[0][0])[i] = 0;
-    __syncthreads();
+__device__ __forceinline__ void place_keys(SortLds& s, int bits, const unsigned (&digit)[ITEMS],
+                                           int here, unsigned (&place)[ITEMS]) {
+    const int lane = threadIdx.x & 63;
+    unsigned* mine = s.wave + (threadIdx.x >> 6) * s.digits;
+    for (int i = lane; i < s.digits; i += 64) mine[i] = 0;
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
-        if (64 * i + lane < here) atomicAdd(&s.wave[wave][digit[i]], 1u);
+        if (64 * i + lane < here) atomicAdd(&mine[digit[i]], 1u);
     __syncthreads();
-    if (threadIdx.x < DIGITS) {
-        unsigned next = s.base[threadIdx.x];
+    if ((int)threadIdx.x < s.digits) {
+        unsigned next = s.base[threadIdx.x], c[SORT_WAVES];
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) c[w] = s.wave[w * s.digits + threadIdx.x];
 #pragma unroll
         for (int w = 0; w < SORT_WAVES; ++w) {
-            const unsigned c = s.wave[w][threadIdx.x];
-            s.wave[w][threadIdx.x] = next;
-            next += c;
+            s.wave[w * s.digits + threadIdx.x] = next;
+            next += c[w];
         }
         s.base[threadIdx.x] = next;
     }
@@ -186,24 +217,25 @@ __device__ __forceinline__ void place_keys(SortLds& s, const unsigned (&digit)[I
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const bool on = 64 * i + lane < here;
-        const unsigned long long peers = same_digit(digit[i], on);
+        const unsigned long long peers = same_digit(digit[i], bits, on);
         const int rank = __popcll(peers & ((1ULL << lane) - 1));
-        place[i] = on ? s.wave[wave][digit[i]] + rank : 0;
+        place[i] = on ? mine[digit[i]] + rank : 0;
         // (a wave's LDS accesses run in their order: all have read before the first one adds)
         __builtin_amdgcn_wave_barrier();
-        if (on && rank == 0) atomicAdd(&s.wave[wave][digit[i]], (unsigned)__popcll(peers));
+        if (on && rank == 0) atomicAdd(&mine[digit[i]], (unsigned)__popcll(peers));
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-// Moves each key and its position to their places by the digit.
+// Moves each key and its position to their places by the digit.  (Counting the next pass's digits
+// here, where the keys arrive, took 40 us in global atomics for the 5 of its own kernel.)
 template <int ITEMS>
 __global__ void __launch_bounds__(SORT_THREADS) move_keys_kernel(SortArgs a) {
-    __shared__ SortLds s;
+    extern __shared__ unsigned sort_lds[];
+    SortLds s(sort_lds, a.bits);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    digit_bases(s, a.counts, a.tiles, blockIdx.x);
-    const long long n0 = (long long)blockIdx.x * a.tile;
-    const long long n1 = min(n0 + a.tile, (long long)a.N);
+    const long long n0 = (long long)blockIdx.x << a.tile_bits;
+    const long long n1 = min(n0 + (1LL << a.tile_bits), (long long)a.N);
     for (long long part = n0; part < n1; part += SORT_THREADS * ITEMS) {
         const long long w0 = part + wave * 64 * ITEMS;
         const int here = (int)min(max(n1 - w0, 0LL), 64LL * ITEMS);
@@ -213,25 +245,27 @@ __global__ void __launch_bounds__(SORT_THREADS) move_keys_kernel(SortArgs a) {
             const int k = 64 * i + lane, n = (int)(w0 + k);
             key[i] = k < here ? key_at(a, n) : 0;
             at[i] = k < here && !a.first ? a.at[n] : (unsigned)n;
-            digit[i] = key[i] >> a.shift & (DIGITS - 1);
+            digit[i] = key[i] >> a.shift & (s.digits - 1);
         }
+        if (part == n0) digit_bases(s, a.counts, a.tiles, blockIdx.x);
         __syncthreads();
-        place_keys(s, digit, here, place);
+        place_keys(s, a.bits, digit, here, place);
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (64 * i + lane < here) {
-                a.keys_to[place[i]] = key[i];
-                a.at_to[place[i]] = at[i];
-                if (a.last && key[i] < (unsigned)a.p.V) a.present[key[i]] = 1;
-            }
+        for (int i = 0; i < ITEMS; ++i) {
+            if (64 * i + lane >= here) continue;
+            a.keys_to[place[i]] = key[i];
+            a.at_to[place[i]] = at[i];
+            if (a.last && key[i] < (unsigned)a.p.V) a.present[key[i]] = 1;
+        }
     }
 }
 
 // All of a short sort in one workgroup: the passes exchange through LDS.
 constexpr int SHORT_ITEMS = 8, SHORT = SORT_THREADS * SHORT_ITEMS;
-__global__ void __launch_bounds__(SORT_THREADS) sort_short_kernel(SortArgs a, int bits) {
-    __shared__ SortLds s;
-    __shared__ unsigned keys[SHORT], ats[SHORT];
+__global__ void __launch_bounds__(SORT_THREADS) sort_short_kernel(SortArgs a, int passes) {
+    extern __shared__ unsigned sort_lds[];
+    SortLds s(sort_lds + 2 * SHORT, a.bits);
+    unsigned *keys = sort_lds, *ats = sort_lds + SHORT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int w0 = wave * 64 * SHORT_ITEMS;
     const int here = min(max(a.N - w0, 0), 64 * SHORT_ITEMS);
@@ -243,33 +277,19 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_short_kernel(SortArgs a, in
         key[i] = n < a.N ? key_at(a, n) : 0;
         at[i] = n;
     }
-    for (int shift = 0; shift < bits; shift += 8) {
+    for (int pass = 0; pass < passes; ++pass) {
         unsigned digit[SHORT_ITEMS], place[SHORT_ITEMS];
-        if (threadIdx.x < DIGITS) s.part[0][0][threadIdx.x] = 0;
+        s.part[threadIdx.x] = 0;        // (one tile, whose counts lie here)
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < SHORT_ITEMS; ++i) {
-            digit[i] = key[i] >> shift & (DIGITS - 1);
-            if (64 * i + lane < here) atomicAdd(&s.part[0][0][digit[i]], 1u);
+            digit[i] = key[i] >> (pass * a.bits) & (s.digits - 1);
+            if (64 * i + lane < here) atomicAdd(&s.part[digit[i]], 1u);
         }
         __syncthreads();
-        // (one tile, whose counts lie in LDS)
-        const unsigned all = threadIdx.x < DIGITS ? s.part[0][0][threadIdx.x] : 0;
-        unsigned sum = all;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const unsigned x = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += x;
-        }
-        if (threadIdx.x < DIGITS && lane == 63) s.scan[wave] = sum;
+        s.set_bases((int)threadIdx.x < s.digits ? s.part[threadIdx.x] : 0, 0);
         __syncthreads();
-        if (threadIdx.x < DIGITS) {
-            unsigned below = 0;
-            for (int w = 0; w < wave; ++w) below += s.scan[w];
-            s.base[threadIdx.x] = below + sum - all;
-        }
-        __syncthreads();
-        place_keys(s, digit, here, place);
+        place_keys(s, a.bits, digit, here, place);
 #pragma unroll
         for (int i = 0; i < SHORT_ITEMS; ++i)
             if (64 * i + lane < here) {
@@ -306,6 +326,7 @@ struct TableArgs {
     const unsigned char* present;
     float *head, *tail;             // [chunks][D]: parts of runs that come from the chunk before
                                     // (or go through it), that begin in a chunk and go on
+    Divisor by_length;
     int N, chunk, chunks;           // positions of a chunk: a multiple of eight
     int lanes, slabs;               // of a team; of SLAB features
     int sum_blocks, zero_blocks;
@@ -344,22 +365,29 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
         }
     };
     bool any = false;                           // acc holds a part of `run`
+    // the next eight rows' places are under way with these eight rows
+    u4v next[4];
+    auto places = [&](int i) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            next[q] = *(const u4v*)(a.keys + i + 4 * q);
+            next[2 + q] = *(const u4v*)(a.at + i + 4 * q);
+        }
+    };
+    places(i0);
     for (int i = i0; i < i1; i += 8) {
-        u4v k[2], n[2];
-        k[0] = *(const u4v*)(a.keys + i);
-        k[1] = *(const u4v*)(a.keys + i + 4);
-        n[0] = *(const u4v*)(a.at + i);
-        n[1] = *(const u4v*)(a.at + i + 4);
+        const u4v k[2] = {next[0], next[1]}, n[2] = {next[2], next[3]};
         if (k[0][0] >= V) break;                // only unused positions are left
-        float x[8][RUN];
+        Eight<TO> r[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const bool on = i + u < i1 && k[u >> 2][u & 3] < V;
             const unsigned at = on ? n[u >> 2][u & 3] : 0;
-            const TO* g = (const TO*)a.grad + (long long)(at / (unsigned)p.L) * p.grad.batch +
-                          (long long)(at % (unsigned)p.L) * p.grad.row + f;
-            load_run(g, on ? left : 0, x[u]);
+            const unsigned b = a.by_length(at), l = at - b * p.L;
+            r[u] = load_run((const TO*)a.grad + (long long)b * p.grad.batch +
+                            (long long)l * p.grad.row, f, D);
         }
+        places(min(i + 8, i1 - 1 & ~7));
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             if (i + u >= i1) break;
@@ -372,8 +400,10 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
                 inside = true;
             }
             any = true;
+            float x[RUN];
+            unpack(r[u], f, D, key < V, x);
 #pragma unroll
-            for (int e = 0; e < RUN; ++e) acc[e] += x[u][e];
+            for (int e = 0; e < RUN; ++e) acc[e] += x[e];
         }
     }
     if (any) flush(i1 >= a.N || a.keys[i1] != run);
@@ -404,22 +434,18 @@ __global__ void __launch_bounds__(256) join_runs_kernel(TableArgs a) {
     }
     const int f = f0 + lane * RUN, left = D - f;
     float acc[RUN] = {};
-    if (wave == 0) load_run(a.tail + (long long)c * D + f, left, acc);
-    int k = c + 1 + wave;
-    for (; k + 12 <= last; k += 16) {
-        float x[4][RUN];
+    if (wave == 0) unpack(load_run(a.tail + (long long)c * D, f, D), f, D, true, acc);
+    for (int k = c + 1 + wave; k <= last; k += 16) {
+        Eight<float> r[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load_run(a.head + (long long)(k + 4 * u) * D + f, left, x[u]);
+        for (int u = 0; u < 4; ++u) r[u] = load_run(a.head + (long long)min(k + 4 * u, last) * D, f, D);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 4; ++u) {
+            float x[RUN];
+            unpack(r[u], f, D, k + 4 * u <= last, x);
 #pragma unroll
-            for (int e = 0; e < RUN; ++e) acc[e] += x[u][e];
-    }
-    for (; k <= last; k += 4) {
-        float x[RUN];
-        load_run(a.head + (long long)k * D + f, left, x);
-#pragma unroll
-        for (int e = 0; e < RUN; ++e) acc[e] += x[e];
+            for (int e = 0; e < RUN; ++e) acc[e] += x[e];
+        }
     }
 #pragma unroll
     for (int e = 0; e < RUN; ++e) part[wave][64 * e + lane] = acc[e];
@@ -435,28 +461,103 @@ __global__ void __launch_bounds__(256) join_runs_kernel(TableArgs a) {
     store_run((TW*)a.dweight + (long long)run * D + f, left, acc);
 }
 
+// ---------------------------------------------------------------------------
+// small tables
+// ---------------------------------------------------------------------------
+// A table of few tokens needs no sort: a workgroup keeps a sum for each token and each of 512
+// features in LDS, where a thread adds to the numbers of its own two features only, in the order
+// of its rows.  The workgroups' tables are added up by rows.hip.
+struct SmallArgs {
+    d2p_token_embedding_params p;
+    Divisor by_length;
+    const void* grad;
+    float* partial;                 // [splits][V][D]
+    int lanes, slabs, rows;         // lanes: threads of a team, two features each; rows of a split
+};
+constexpr int SMALL_ROWS = 512;     // whose tokens are looked up at a time
+
+template <class TO> __global__ void __launch_bounds__(256) table_grad_small_kernel(SmallArgs a) {
+    constexpr int ROWS = 16;        // in flight
+    struct Two { TO v[2]; };
+    extern __shared__ float sums[]; // [V][2][256], and the tokens
+    const d2p_token_embedding_params& p = a.p;
+    int* tokens = (int*)(sums + p.V * SLAB);
+    const int me = threadIdx.x, teams = 256 / a.lanes, team = me / a.lanes;
+    const int split = blockIdx.x / a.slabs;
+    const int f = blockIdx.x % a.slabs * SLAB + (me & (a.lanes - 1)) * 2;
+    const long long N = (long long)p.B * p.L;
+    const int r0 = min((long long)split * a.rows, N), r1 = min((long long)r0 + a.rows, N);
+    // behind the features' end the last two are read; of a lone last one, it and the one before
+    const int f0 = min(f, p.D - 2);
+    const bool lone = f == p.D - 1;
+    for (int i = 0; i < p.V * 2; ++i) sums[i * 256 + me] = 0.0f;
+    for (int part = r0; part < r1; part += SMALL_ROWS) {
+        const int rows = min(SMALL_ROWS, r1 - part);
+        __syncthreads();
+        for (int i = me; i < rows; i += 256) tokens[i] = token_at(p, a.by_length, part + i);
+        __syncthreads();
+        for (int r = team; r < rows; r += ROWS * teams) {
+            Two x[ROWS];
+            int t[ROWS];
+#pragma unroll
+            for (int u = 0; u < ROWS; ++u) {
+                const int i = min(r + u * teams, rows - 1);
+                const unsigned n = part + i, b = a.by_length(n);
+                x[u] = *(const Two*)((const TO*)a.grad + (long long)b * p.grad.batch +
+                                     (long long)(n - b * p.L) * p.grad.row + f0);
+                t[u] = r + u * teams < rows ? tokens[i] : ABSENT;
+            }
+#pragma unroll
+            for (int u = 0; u < ROWS; ++u) {
+                if (t[u] < 0) continue;
+                float* to = sums + t[u] * SLAB + me;
+                // (LDS additions as such, ds_add_f32, take 300 cycles a wave)
+                const float s0 = to[0], s1 = to[256];
+                to[0] = s0 + (float)(lone ? x[u].v[1] : x[u].v[0]);
+                to[256] = s1 + (float)x[u].v[1];
+            }
+        }
+    }
+    __syncthreads();
+    // the teams' tables, in order
+    float* to = a.partial + (long long)split * p.V * p.D;
+    for (int v = team; v < p.V; v += teams) {
+        const float* from = sums + v * SLAB + (me & (a.lanes - 1));
+        float s0 = 0.0f, s1 = 0.0f;
+        for (int k = 0; k < 256; k += a.lanes) {
+            s0 += from[k];
+            s1 += from[k + 256];
+        }
+        if (f < p.D) to[(long long)v * p.D + f] = s0;
+        if (f + 1 < p.D) to[(long long)v * p.D + f + 1] = s1;
+    }
+}
+
 namespace {
 
 int check(const d2p_token_embedding_params* p) {
     D2P_REQUIRE(p != nullptr, "null parameters");
     D2P_REQUIRE(known_pair(p->weight_dtype, p->dtype),
                 "unknown element types, or a pair other than equal ones and 16 bits beside float32");
-    D2P_REQUIRE(p->B >= 0 && p->L >= 0 && p->V >= 0, "negative size");
+    D2P_REQUIRE(p->B >= 0 && p->L >= 0, "negative size");
     D2P_REQUIRE((long long)p->B * p->L < 1LL << 31, "too many tokens");
-    D2P_REQUIRE(p->V < 0x7fffffff, "too many rows");
-    D2P_REQUIRE(p->D >= 1 && p->D <= 1 << 20, "features must be between 1 and 2^20");
+    D2P_REQUIRE(p->V >= 1 && p->V < 0x7fffffff, "the table must have between 1 and 2^31 - 2 rows");
+    D2P_REQUIRE(p->D >= RUN && p->D <= 1 << 20, "features must be between 8 and 2^20");
     D2P_REQUIRE(p->token_bytes == 4 || p->token_bytes == 8, "tokens must have 4 or 8 bytes");
-    D2P_REQUIRE(p->padding >= -1 && p->padding < std::max(p->V, 1), "padding must be a token, or -1");
+    D2P_REQUIRE(p->padding >= -1 && p->padding < p->V, "padding must be a token, or -1");
     D2P_REQUIRE(p->scale > -__builtin_inff() && p->scale < __builtin_inff(), "scale must be finite");
     return D2P_OK;
 }
 
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
+constexpr int SMALL = 32;
+
 // How the backward pass splits its work, and its workspace.
 struct Plan {
-    int N, bits, passes, tile, tiles;
+    int N, bits, passes, tile_bits, tiles;
     bool short_sort;
+    int splits;             // of a small table's rows; 0 for another table
     int lanes, slabs, chunk, chunks;
     size_t keys, counts, present, parts, total;
 
@@ -464,14 +565,24 @@ struct Plan {
         N = p.B * p.L;
         bits = 1;
         while (bits < 31 && (p.V >> bits) != 0) ++bits;     // of V, which stands for no token
-        passes = (bits + 7) / 8;
+        passes = cdiv(bits, MOST_BITS);
+        bits = cdiv(bits, passes);
         short_sort = N <= SHORT && p.V <= 1 << 20;
-        const int part = 2 * SORT_THREADS;
-        tiles = std::max(1, std::min(MOST_TILES, cdiv(N, part)));
-        tile = std::max(1, cdiv(cdiv(N, tiles), part)) * part;
-        tiles = std::max(1, cdiv(N, tile));
+        tile_bits = 11;         // two keys a thread
+        while (cdiv(N, 1 << tile_bits) > MOST_TILES) ++tile_bits;
+        tiles = std::max(1, cdiv(N, 1 << tile_bits));
         lanes = std::min(team_of(p.D), 64);
         slabs = cdiv(p.D, SLAB);
+        splits = 0;
+        if (p.V <= SMALL && (long long)p.V * p.D <= 1 << 24) {
+            // workgroups that the card's LDS holds at a time, each with more rows than its table has
+            const int groups = 256 * std::min(8, 156 / (2 * p.V));
+            splits = std::max(1, std::min(groups / slabs, N / (2 * p.V)));
+            if (splits > 256) splits -= splits % 256;       // as many for each compute unit
+            if (N) splits = cdiv(N, cdiv(N, splits));
+            total = (size_t)splits * p.V * p.D * 4;
+            return;
+        }
         // chunks of 64 positions where they give the card's waves work, shorter ones where
         // positions are few, longer ones where the joins of long runs would be
         const long long waves = (long long)N * slabs * lanes / 64;
@@ -479,12 +590,37 @@ struct Plan {
         while (chunk < 256 && waves / chunk > 4096) chunk *= 2;
         chunks = cdiv(N, chunk);
         keys = round16(((size_t)N + 8) * 4);
-        counts = (size_t)tiles * DIGITS * 4;
+        counts = round16(((size_t)tiles << bits) * 4);
         present = round16(p.V);
         parts = round16((size_t)chunks * p.D * 4);
         total = 4 * keys + counts + present + 2 * parts;
     }
 };
+
+int launch_small(const d2p_token_embedding_params& p, const Plan& plan, const void* grad,
+                 float* partial, void* dweight, hipStream_t st) {
+    int lanes = 1;
+    while (lanes < 256 && 2 * lanes < p.D) lanes *= 2;
+    const SmallArgs a{p, Divisor(p.L), grad, partial, lanes, plan.slabs,
+                      plan.N ? cdiv(plan.N, plan.splits) : 0};
+    SumJobs jobs;
+    jobs.init(p.V * p.D);
+    jobs.scale = p.scale;
+    jobs.add(partial, dweight, p.weight_dtype, plan.N ? plan.splits : 0, 1);
+    if (plan.N)
+        D2P_TRY(with_pair(p.dtype, p.dtype, [&](auto to, auto) {
+            using TO = typename decltype(to)::type;
+            static LdsAllowed known;
+            D2P_TRY(allow_lds((const void*)table_grad_small_kernel<TO>, known));
+            D2P_LAUNCH("token_embedding_backward", table_grad_small_kernel<TO>,
+                       dim3(plan.splits * plan.slabs), dim3(256),
+                       (p.V * SLAB + SMALL_ROWS) * sizeof(float), st,
+                       a);
+            D2P_HIP(hipGetLastError());
+            return D2P_OK;
+        }));
+    return launch_sum_rows("token_embedding_sum", jobs, st);
+}
 
 int launch_sort(const d2p_token_embedding_params& p, const Plan& plan, char* ws, TableArgs& t,
                 hipStream_t st) {
@@ -492,36 +628,40 @@ int launch_sort(const d2p_token_embedding_params& p, const Plan& plan, char* ws,
     unsigned* at[2] = {(unsigned*)(ws + 2 * plan.keys), (unsigned*)(ws + 3 * plan.keys)};
     SortArgs a{};
     a.p = p;
+    a.by_length = Divisor(p.L);
     a.N = plan.N;
     a.tiles = plan.tiles;
-    a.tile = plan.tile;
-    a.first = a.last = 1;
+    a.tile_bits = plan.tile_bits;
+    a.bits = plan.bits;
+    a.first = 1;
     a.keys_to = key[0];
     a.at_to = at[0];
     a.counts = (unsigned*)(ws + 4 * plan.keys);
     a.present = (unsigned char*)(ws + 4 * plan.keys + plan.counts);
     t.present = a.present;
-    t.keys = key[0];
-    t.at = at[0];
     if (plan.short_sort) {
-        D2P_LAUNCH("token_sort", sort_short_kernel, dim3(1), dim3(SORT_THREADS), 0, st, a, plan.bits);
+        static LdsAllowed known;
+        D2P_TRY(allow_lds((const void*)sort_short_kernel, known));
+        D2P_LAUNCH("token_sort", sort_short_kernel, dim3(1), dim3(SORT_THREADS),
+                   2 * SHORT * sizeof(unsigned) + SortLds::bytes(plan.bits), st, a, plan.passes);
         D2P_HIP(hipGetLastError());
-        return D2P_OK;
     }
-    const int clearing = (int)std::min<long long>(256, p.V / (64 << 10) + 1);
-    for (int n = 0; n < plan.passes; ++n) {
+    for (int n = 0; n < plan.passes && !plan.short_sort; ++n) {
         a.first = n == 0;
         a.last = n == plan.passes - 1;
-        a.shift = 8 * n;
+        a.shift = plan.bits * n;
         a.keys = key[(n + 1) & 1];
         a.at = at[(n + 1) & 1];
         a.keys_to = key[n & 1];
         a.at_to = at[n & 1];
-        D2P_LAUNCH("token_sort_count", count_digits_kernel,
-                   dim3(std::max(plan.tiles, a.first ? clearing : 1)), dim3(SORT_THREADS), 0, st, a);
+        const int clearing = a.first ? (int)std::min<long long>(256, p.V / (64 << 10) + 1) : 1;
+        D2P_LAUNCH("token_sort_count", count_digits_kernel, dim3(std::max(plan.tiles, clearing)),
+                   dim3(SORT_THREADS), 0, st, a);
         D2P_HIP(hipGetLastError());
-        D2P_LAUNCH("token_sort_move", move_keys_kernel<2>, dim3(plan.tiles), dim3(SORT_THREADS), 0,
-                   st, a);
+        static LdsAllowed known;
+        D2P_TRY(allow_lds((const void*)move_keys_kernel<2>, known));
+        D2P_LAUNCH("token_sort_move", move_keys_kernel<2>, dim3(plan.tiles), dim3(SORT_THREADS),
+                   SortLds::bytes(plan.bits), st, a);
         D2P_HIP(hipGetLastError());
     }
     t.keys = a.keys_to;
@@ -540,8 +680,8 @@ extern "C" int d2p_token_embedding(const d2p_token_embedding_params* p, const vo
                                    void* out, void* stream) {
     D2P_TRY(check(p));
     if ((long long)p->B * p->L == 0) return D2P_OK;
-    D2P_REQUIRE(p->tokens && out && (weight || p->V == 0), "null pointer argument");
-    EmbedArgs a{*p, weight, out, std::min(team_of(p->D), 64)};
+    D2P_REQUIRE(p->tokens && out && weight, "null pointer argument");
+    EmbedArgs a{*p, weight, out, std::min(team_of(p->D), 64), Divisor(p->L)};
     const int most = 8 * std::max(device_cus(), 1);
     const int grid = std::min(cdiv(p->B * p->L, 256 / a.lanes), most);
     return with_pair(p->weight_dtype, p->dtype, [&](auto tw, auto to) {
@@ -555,7 +695,7 @@ extern "C" int d2p_token_embedding(const d2p_token_embedding_params* p, const vo
 }
 
 extern "C" size_t d2p_token_embedding_backward_workspace_bytes(const d2p_token_embedding_params* p) {
-    if (!p || p->B < 0 || p->L < 0 || p->V < 0 || p->D < 1 || p->D > 1 << 20 ||
+    if (!p || p->B < 0 || p->L < 0 || p->V < 1 || p->D < RUN || p->D > 1 << 20 ||
         p->V >= 0x7fffffff || (long long)p->B * p->L >= 1LL << 31)
         return 0;
     return Plan(*p).total;
@@ -565,17 +705,19 @@ extern "C" int d2p_token_embedding_backward(const d2p_token_embedding_params* p,
                                             void* dweight, void* workspace, size_t workspace_bytes,
                                             void* stream) {
     D2P_TRY(check(p));
-    if (p->V == 0) return D2P_OK;
     const bool rows = (long long)p->B * p->L > 0;
     D2P_REQUIRE(dweight && (!rows || (p->tokens && grad)), "null pointer argument");
     const Plan plan(*p);
     D2P_REQUIRE(workspace && workspace_bytes >= plan.total, "workspace too small");
     D2P_REQUIRE(((uintptr_t)workspace & 15) == 0, "the workspace must be aligned to 16 bytes");
     hipStream_t st = (hipStream_t)stream;
+    if (plan.splits)
+        return launch_small(*p, plan, grad, (float*)workspace, dweight, st);
     TableArgs a{};
     a.p = *p;
     a.grad = grad;
     a.dweight = dweight;
+    a.by_length = Divisor(p->L);
     a.N = plan.N;
     a.lanes = plan.lanes;
     a.slabs = plan.slabs;

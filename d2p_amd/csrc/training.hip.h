@@ -16,28 +16,64 @@ template <class T> struct Eight {
     T v[RUN];
 };
 
-// x = the first `left` of eight numbers from p on (left may be zero or less, or past eight),
-// zeros behind them
-template <class T> __device__ __forceinline__ void load_run(const T* p, int left, float* x) {
-    if (left >= RUN) {
-        const Eight<T> a = *(const Eight<T>*)p;
+// Eight numbers moved `by` (0 to 7) places to the front, zeros behind them: shifts by four, two
+// and one.
+template <class T> __device__ __forceinline__ Eight<T> to_front(const Eight<T>& a, int by) {
+    constexpr int W = sizeof(Eight<T>) / 4, PER = RUN / W;      // words, numbers of one
+    struct Words { unsigned v[W]; };
+    Words w = bits<Words>(a);
 #pragma unroll
-        for (int e = 0; e < RUN; ++e) x[e] = (float)a.v[e];
-    } else {
+    for (int step = 4; step >= PER; step /= 2) {
+        const bool on = by & step;
 #pragma unroll
-        for (int e = 0; e < RUN; ++e) x[e] = e < left ? (float)p[e] : 0.0f;
+        for (int i = 0; i < W; ++i) {
+            const unsigned next = i + step / PER < W ? w.v[i + step / PER] : 0;
+            w.v[i] = on ? next : w.v[i];
+        }
     }
+    if constexpr (PER == 2) {
+        const int half = by & 1 ? 16 : 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            w.v[i] = __builtin_amdgcn_alignbit(i + 1 < W ? w.v[i + 1] : 0, w.v[i], half);
+    }
+    return bits<Eight<T>>(w);
 }
+
+// The eight numbers of a row of D (eight at least) from `at` on, in two steps, so that all loads
+// of a turn are under way before the first is waited for: load_run reads eight numbers of the
+// row whatever `at` is, at the row's end the last eight, which unpack then moves into place.
+// (A branch around each load, and its conversion behind it, made the loads wait for each other.)
+template <class T> __device__ __forceinline__ Eight<T> load_run(const T* row, int at, int D) {
+    return *(const Eight<T>*)(row + min(at, D - RUN));
+}
+// x = the numbers; zeros behind the row's end, and where the row is not wanted.  EVEN: D is known to
+// be a multiple of eight.
+template <bool EVEN = false, class T>
+__device__ __forceinline__ void unpack(const Eight<T>& a, int at, int D, bool wanted, float* x) {
+    Eight<T> b = a;
+    if (!EVEN && D % RUN) b = to_front(a, min(max(at - (D - RUN), 0), RUN - 1));
+    const bool on = wanted && at < D;
+#pragma unroll
+    for (int e = 0; e < RUN; ++e) x[e] = on ? (float)b.v[e] : 0.0f;
+}
+
+template <class T, int N> struct Few {
+    T v[N];
+};
 template <class T> __device__ __forceinline__ void store_run(T* p, int left, const float* x) {
+    Eight<T> a;
+#pragma unroll
+    for (int e = 0; e < RUN; ++e) a.v[e] = (T)x[e];
     if (left >= RUN) {
-        Eight<T> a;
-#pragma unroll
-        for (int e = 0; e < RUN; ++e) a.v[e] = (T)x[e];
         *(Eight<T>*)p = a;
-    } else {
-#pragma unroll
-        for (int e = 0; e < RUN; ++e)
-            if (e < left) p[e] = (T)x[e];
+    } else if (left > 0) {      // four, two and one
+        const bool four = left & 4, two = left & 2;
+        if (four) *(Few<T, 4>*)p = {a.v[0], a.v[1], a.v[2], a.v[3]};
+        if (two)
+            *(Few<T, 2>*)(p + (left & 4)) = {four ? a.v[4] : a.v[0], four ? a.v[5] : a.v[1]};
+        if (left & 1)
+            p[left & 6] = four ? (two ? a.v[6] : a.v[4]) : (two ? a.v[2] : a.v[0]);
     }
 }
 // one number whose type is known only at run time
@@ -77,6 +113,32 @@ inline int team_of(int D) {
     return n;
 }
 
+// s / n, n a whole number below 2^24: the product with 1 / n and what it leaves, which gives
+// exact quotients exactly (a mean of equal numbers is that number).
+__device__ __forceinline__ float divided(float s, float n) {
+    const float per = __builtin_amdgcn_rcpf(n), q = s * per;
+    return fmaf(fmaf(-q, n, s), per, q);
+}
+// 1 / sqrt(x) within two roundings, where x is below the normal numbers too
+__device__ __forceinline__ float inverse_root(float x) {
+    const bool tiny = x < 0x1p-96f;
+    return __builtin_amdgcn_rsqf(tiny ? x * 0x1p96f : x) * (tiny ? 0x1p48f : 1.0f);
+}
+
+// n / d for n below 2^31, by a product (T. Granlund and P. Montgomery, "Division by invariant
+// integers using multiplication", PLDI 1994).
+struct Divisor {
+    unsigned d, magic, shift;
+    Divisor() = default;
+    explicit Divisor(int d_) : d(d_ > 0 ? d_ : 1), magic(0), shift(0) {
+        while ((1ULL << shift) < d) ++shift;
+        magic = (unsigned)((((1ULL << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ unsigned operator()(unsigned n) const {
+        return (__umulhi(n, magic) + n) >> shift;
+    }
+};
+
 // The threads that hold one row.  Up to 64 lanes of one wave, or (WIDE) whole waves, which
 // exchange their sums through LDS: two sets of them in turn, so that one barrier a sum does.
 template <bool WIDE> struct Team {
@@ -95,19 +157,20 @@ template <bool WIDE> struct Team {
     __device__ __forceinline__ float sum(float a) {
         return WIDE ? exchange(group_sum(a, 64), 0.0f).x : group_sum(a, lanes);
     }
-    // Mean and the sum of squares around it of D numbers, x[e] being there for e < left: in two
-    // passes over the registers, each wave around a mean of its own.
-    __device__ __forceinline__ float2 spread(const float* x, int left, int D) {
+    // Mean and the sum of squares around it of D numbers, `there` being 1 for the lane's numbers
+    // and 0 (x too) behind the row's end: in two passes over the registers, each wave around a
+    // mean of its own.
+    __device__ __forceinline__ float2 spread(const float* x, const float* there, int D) {
         float s = 0.0f, m2 = 0.0f;
 #pragma unroll
         for (int e = 0; e < RUN; ++e) s += x[e];
         const int members = WIDE ? 64 : lanes;
         const int count = WIDE ? min(max(D - (n & ~63) * RUN, 0), 64 * RUN) : D;
         s = group_sum(s, members);
-        const float mean = s / max(count, 1);
+        const float mean = divided(s, (float)max(count, 1));
 #pragma unroll
         for (int e = 0; e < RUN; ++e) {
-            const float c = e < left ? x[e] - mean : 0.0f;
+            const float c = fmaf(-mean, there[e], x[e]);
             m2 += c * c;
         }
         m2 = group_sum(m2, members);
@@ -117,10 +180,10 @@ template <bool WIDE> struct Team {
         const int waves = lanes >> 6;
         float total = 0.0f, squares = 0.0f;
         for (int w = 0; w < waves; ++w) total += at[w].x;
-        const float common = total / D;
+        const float common = divided(total, (float)D);
         for (int w = 0; w < waves; ++w) {
             const int c = min(max(D - w * 64 * RUN, 0), 64 * RUN);
-            const float d = c ? at[w].x / c - common : 0.0f;
+            const float d = c ? divided(at[w].x, (float)c) - common : 0.0f;
             squares += at[w].y + c * d * d;
         }
         return {common, squares};
@@ -159,9 +222,11 @@ struct SumJobs {
     SumJob job[6];
     int jobs, D, tiles;                // tiles of 64 numbers
     int blocks;
+    float scale;                       // of all results
 
     void init(int D_) {
         D = D_;
+        scale = 1.0f;
         tiles = cdiv(D_, 64);
         jobs = blocks = 0;
     }

@@ -23,13 +23,11 @@ void check_on(const Tensor& t, const Tensor& like, const char* name) {
 
 // Strides of a [.., row, feature] tensor whose features are adjacent (a copy where they are not).
 Tensor adjacent_rows(const Tensor& t) {
-    return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+    return t.stride(-1) == 1 ? t : t.contiguous();
 }
 d2p_row_strides row_strides(const Tensor& t) {
     return {t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
 }
-
-Tensor nothing(const Tensor& like) { return torch::empty({0}, like.options()); }
 
 // ---------------------------------------------------------------------------
 // token embedding
@@ -54,8 +52,9 @@ EmbedInputs embed_inputs(const Tensor& tokens, const OptTensor& lengths, double 
     TORCH_CHECK((int64_t)p.B * p.L < int64_t(1) << 31, "too many tokens: ", tokens.numel());
     p.V = dim32(rows, "rows of the weight");
     p.D = dim32(features, "features");
-    TORCH_CHECK(p.D >= 1 && p.D <= 1 << 20, "features must be between 1 and 2^20, got ", p.D);
-    TORCH_CHECK(p.V < std::numeric_limits<int>::max(), "too many rows: ", p.V);
+    TORCH_CHECK(p.D >= 8 && p.D <= 1 << 20, "features must be between 8 and 2^20, got ", p.D);
+    TORCH_CHECK(p.V >= 1 && p.V < std::numeric_limits<int>::max(),
+                "weight must have between 1 and 2^31 - 2 rows, got ", p.V);
     p.weight_dtype = weight_dtype;
     p.dtype = dtype;
     TORCH_CHECK(weight_dtype == dtype || weight_dtype == D2P_FLOAT32,
@@ -72,7 +71,7 @@ EmbedInputs embed_inputs(const Tensor& tokens, const OptTensor& lengths, double 
         in.lengths = lengths->contiguous();
         p.lengths = in.lengths.data_ptr<int>();
     }
-    TORCH_CHECK(padding >= -1 && padding < std::max(p.V, 1), "padding must be a token of ", p.V,
+    TORCH_CHECK(padding >= -1 && padding < p.V, "padding must be a token of ", p.V,
                 ", got ", padding);
     p.padding = padding;
     TORCH_CHECK(std::isfinite(scale) && std::isfinite((float)scale), "scale must be finite, got ",
@@ -208,7 +207,7 @@ ResidualInputs residual_inputs(const Tensor& x, const OptTensor& weight, const O
                 x.scalar_type());
     p.B = dim32(x.size(0), "batch size");
     p.L = dim32(x.size(1), "length");
-    TORCH_CHECK(x.size(2) >= 1 && x.size(2) <= 8192, "features must be between 1 and 8192, got ",
+    TORCH_CHECK(x.size(2) >= 8 && x.size(2) <= 8192, "features must be between 8 and 8192, got ",
                 x.size(2));
     p.D = (int)x.size(2);
     TORCH_CHECK((int64_t)p.B * p.L < int64_t(1) << 31, "too many rows: ", x.sizes());
@@ -261,10 +260,10 @@ ThreeTensors residual_norm_forward(const Tensor& x_, const OptTensor& y_, const 
     in.p.x = row_strides(x);
     if (block) in.p.y = row_strides(y);
     in.p.with_y = block;
-    Tensor h = block ? torch::empty(x.sizes(), x.options()) : nothing(x);
-    Tensor n = norm ? torch::empty(x.sizes(), x.options().dtype(dtype)) : nothing(x);
+    Tensor h = block ? torch::empty(x.sizes(), x.options()) : Tensor();
+    Tensor n = norm ? torch::empty(x.sizes(), x.options().dtype(dtype)) : Tensor();
     Tensor st = stats ? torch::empty({x.size(0), x.size(1), 4}, x.options().dtype(torch::kFloat32))
-                      : torch::empty({0}, x.options().dtype(torch::kFloat32));
+                      : Tensor();
     D2P_CALL(d2p_residual_norm(&in.p, x.data_ptr(), block ? y.data_ptr() : nullptr,
                                block ? h.data_ptr() : nullptr, norm ? n.data_ptr() : nullptr,
                                stats ? st.data_ptr<float>() : nullptr, current_stream()));
@@ -273,8 +272,8 @@ ThreeTensors residual_norm_forward(const Tensor& x_, const OptTensor& y_, const 
 
 using SevenTensors = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-// h: the forward's (x itself where there is no y).  dy comes back empty where it equals dx, and
-// every gradient that `wanted` (bits: gate, then the four vectors) leaves out.
+// h: the forward's for float32, x for 16 bits and where there is no y.  dy comes back undefined where it equals dx, and
+// so does every gradient that `wanted` (bits: gate, then the four vectors) leaves out.
 SevenTensors residual_norm_backward(const OptTensor& dh_, const OptTensor& dn_, const Tensor& h_,
                                     const OptTensor& y_, const Tensor& stats,
                                     const OptTensor& weight, const OptTensor& bias,
@@ -286,7 +285,8 @@ SevenTensors residual_norm_backward(const OptTensor& dh_, const OptTensor& dn_, 
     c10::hip::HIPGuardMasqueradingAsCUDA guard(h_.device());
     auto in = residual_inputs(h_, weight, bias, post_weight, post_bias, gate, norm, post_norm,
                               scale, residual_scale, eps, dtype);
-    const Tensor h = block ? h_.contiguous() : adjacent_rows(h_);
+    const Tensor h = block && h_.scalar_type() == torch::kFloat32 ? h_.contiguous()
+                                                                  : adjacent_rows(h_);
     in.p.x = row_strides(h);
     in.p.with_y = block;
     Tensor dh, dn, y;
@@ -312,11 +312,9 @@ SevenTensors residual_norm_backward(const OptTensor& dh_, const OptTensor& dn_, 
     const bool same = block && !post_norm && !given(gate) && scale == residual_scale &&
                       h.scalar_type() == dtype;
     Tensor dx = torch::empty(h.sizes(), h.options());
-    Tensor dy = block && !same ? torch::empty(h.sizes(), h.options().dtype(dtype)) : nothing(h);
+    Tensor dy = block && !same ? torch::empty(h.sizes(), h.options().dtype(dtype)) : Tensor();
     auto of = [&](const OptTensor& v, int bit) {
-        return given(v) && (wanted >> bit & 1) ? torch::empty(v->sizes(), v->options().memory_format(
-                                                     at::MemoryFormat::Contiguous))
-                                               : nothing(h);
+        return given(v) && (wanted >> bit & 1) ? torch::empty(v->sizes(), v->options()) : Tensor();
     };
     Tensor dgate = of(gate, 0), dw = of(weight, 1), db = of(bias, 2), dpw = of(post_weight, 3),
            dpb = of(post_bias, 4);
@@ -348,12 +346,15 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
                                const OptTensor& gate, int64_t norm, int64_t post_norm, double scale,
                                double residual_scale, double eps, at::ScalarType dtype) {
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [h, n, stats] = call_residual(x, y, weight, bias, post_weight, post_bias, gate, norm,
-                                           post_norm, scale, residual_scale, eps, dtype, true);
+        Tensor h, n, stats;
+        std::tie(h, n, stats) =
+            call_residual(x, y, weight, bias, post_weight, post_bias, gate, norm, post_norm, scale,
+                          residual_scale, eps, dtype, true);
         auto wants = [](const OptTensor& t) { return given(t) && t->requires_grad(); };
-        // y enters the gradients through its own norm and the gate's alone
-        const bool keep_y = post_norm || wants(gate);
-        ctx->save_for_backward({given(y) ? h : x, keep_y ? y.value_or(Tensor()) : Tensor(), stats,
+        // y enters the gradients through its own norm, the gate's, and h where that is rounded
+        const bool wide = x.scalar_type() == torch::kFloat32;
+        const bool keep_y = post_norm || wants(gate) || (norm && !wide);
+        ctx->save_for_backward({given(y) && wide ? h : x, keep_y ? y.value_or(Tensor()) : Tensor(), stats,
                                 weight.value_or(Tensor()), bias.value_or(Tensor()),
                                 post_weight.value_or(Tensor()), post_bias.value_or(Tensor()),
                                 gate.value_or(Tensor())});
@@ -367,6 +368,9 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
         ctx->saved_data["wanted"] = int64_t(wants(gate)) | wants(weight) << 1 | wants(bias) << 2 |
                                     wants(post_weight) << 3 | wants(post_bias) << 4;
         ctx->set_materialize_grads(false);
+        // (a function's results are tensors)
+        for (Tensor* t : {&h, &n})
+            if (!t->defined()) *t = torch::empty({0}, x.options());
         return {h, n};
     }
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
@@ -385,14 +389,13 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
                     saved(s[4]), saved(s[5]), saved(s[6]), saved(s[7]), d["norm"].toInt(),
                     d["post_norm"].toInt(), d["scale"].toDouble(), d["residual_scale"].toDouble(),
                     d["eps"].toDouble(), (at::ScalarType)d["dtype"].toInt(), block, wanted);
-        auto of = [&](int bit, const Tensor& t) { return wanted >> bit & 1 ? t : Tensor(); };
-        out[0] = dx;
-        if (block) out[1] = dy.dim() == 3 ? dy : dx;
-        out[2] = of(1, dw);
-        out[3] = of(2, db);
-        out[4] = of(3, dpw);
-        out[5] = of(4, dpb);
-        out[6] = of(0, dgate);
+                out[0] = dx;
+        if (block) out[1] = dy.defined() ? dy : dx;
+        out[2] = dw;
+        out[3] = db;
+        out[4] = dpw;
+        out[5] = dpb;
+        out[6] = dgate;
         return out;
     }
 };
@@ -459,7 +462,7 @@ Tensor global_norm(at::TensorList ts) {
     copies.reserve(ts.size());
     const auto list = tensor_list_of(ts, copies);
     Tensor norm = torch::empty({}, ts[0].options().dtype(torch::kFloat32));
-    const size_t bytes = d2p_global_norm_workspace_bytes();
+    const size_t bytes = d2p_global_norm_workspace_bytes((int)list.size());
     Tensor ws = workspace(bytes, ts[0]);
     D2P_CALL(d2p_global_norm(list.data(), (int)list.size(), norm.data_ptr<float>(), ws.data_ptr(),
                              bytes, current_stream()));
@@ -469,27 +472,49 @@ Tensor global_norm(at::TensorList ts) {
 Tensor clip_lists(std::vector<d2p_tensor>& list, const Tensor& like, double max_norm) {
     TORCH_CHECK(max_norm >= 0, "max_norm must not be negative, got ", max_norm);
     Tensor norm = torch::empty({}, like.options().dtype(torch::kFloat32));
-    const size_t bytes = d2p_global_norm_workspace_bytes();
+    const size_t bytes = d2p_global_norm_workspace_bytes((int)list.size());
     Tensor ws = workspace(bytes, like);
     D2P_CALL(d2p_clip_by_norm(list.data(), (int)list.size(), max_norm, norm.data_ptr<float>(),
                               ws.data_ptr(), bytes, current_stream()));
     return norm;
 }
 
+// Contiguous memory for results, or, for a dense source, memory in its order.  One allocation
+// holds them all, each at a multiple of 256 bytes: one apiece takes the host a microsecond each.
+std::vector<Tensor> results_for(at::TensorList ts, std::vector<d2p_tensor>& list) {
+    int64_t bytes = 0;
+    for (const auto& t : list) bytes += (t.n * (t.dtype == D2P_FLOAT32 ? 4 : 2) + 255) / 256 * 256;
+    Tensor all = workspace(bytes, ts[0]);
+    std::vector<Tensor> out;
+    out.reserve(ts.size());
+    int64_t at = 0;
+    for (size_t i = 0; i < ts.size(); ++i) {
+        const Tensor& t = ts[i];
+        const int64_t size = t.element_size();
+        auto r = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()),
+                                                          all.key_set(), t.dtype());
+        auto* impl = r.unsafeGetTensorImpl();
+        if (t.is_non_overlapping_and_dense()) {
+            impl->set_sizes_and_strides(t.sizes(), t.strides(), at / size);
+        } else {
+            impl->set_storage_offset(at / size);
+            impl->set_sizes_contiguous(t.sizes());
+        }
+        list[i].dst = (char*)all.data_ptr() + at;
+        at += (list[i].n * size + 255) / 256 * 256;
+        out.push_back(std::move(r));
+    }
+    return out;
+}
+
 std::tuple<std::vector<Tensor>, Tensor> clip_gradients(at::TensorList ts, double max_norm) {
     TORCH_CHECK(!ts.empty(), "need at least one tensor");
     TORCH_CHECK(ts[0].is_cuda(), "every tensor must be a CUDA tensor");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(ts[0].device());
-    std::vector<Tensor> copies, out;
+    std::vector<Tensor> copies;
     copies.reserve(ts.size());
-    out.reserve(ts.size());
     auto list = tensor_list_of(ts, copies);
-    for (size_t i = 0; i < list.size(); ++i) {
-        out.push_back(ts[i].is_non_overlapping_and_dense()
-                          ? torch::empty_strided(ts[i].sizes(), ts[i].strides(), ts[i].options())
-                          : torch::empty(ts[i].sizes(), ts[i].options()));
-        list[i].dst = out.back().data_ptr();
-    }
+    std::vector<Tensor> out = results_for(ts, list);
     Tensor norm = clip_lists(list, ts[0], max_norm);
     return {std::move(out), norm};
 }
@@ -497,31 +522,26 @@ std::tuple<std::vector<Tensor>, Tensor> clip_gradients(at::TensorList ts, double
 // Results that share memory with each other, or with a source other than their own, would be
 // read after they are written.
 void check_apart(const std::vector<d2p_tensor>& list) {
-    struct Range {
-        const char *from, *to;
-        size_t of;
-        bool result;
+    using Range = std::pair<uintptr_t, uintptr_t>;
+    auto range = [](const void* from, const d2p_tensor& t) {
+        return Range((uintptr_t)from, (uintptr_t)from + t.n * (t.dtype == D2P_FLOAT32 ? 4 : 2));
     };
-    std::vector<Range> ranges;
-    ranges.reserve(2 * list.size());
-    for (size_t i = 0; i < list.size(); ++i) {
-        const auto& t = list[i];
-        const long long bytes = t.n * (t.dtype == D2P_FLOAT32 ? 4 : 2);
-        if (!bytes) continue;
-        const char *s = (const char*)t.src, *d = (const char*)t.dst;
-        ranges.push_back({d, d + bytes, i, true});
-        if (s != d) ranges.push_back({s, s + bytes, i, false});
+    std::vector<Range> results;
+    results.reserve(list.size());
+    for (const auto& t : list)
+        if (t.n) results.push_back(range(t.dst, t));
+    if (!std::is_sorted(results.begin(), results.end())) std::sort(results.begin(), results.end());
+    bool apart = true;
+    for (size_t i = 1; i < results.size(); ++i) apart &= results[i - 1].second <= results[i].first;
+    for (const auto& t : list) {
+        if (!t.n || t.src == t.dst) continue;
+        const Range r = range(t.src, t);
+        // the first result that ends after the source begins
+        auto it = std::upper_bound(results.begin(), results.end(), r.first,
+                                   [](uintptr_t x, const Range& y) { return x < y.second; });
+        apart &= it == results.end() || it->first >= r.second;
     }
-    std::sort(ranges.begin(), ranges.end(),
-              [](const Range& a, const Range& b) { return a.from < b.from; });
-    const Range *last = nullptr, *result = nullptr;     // that reach furthest
-    for (const Range& r : ranges) {
-        const Range* other = r.result ? last : result;
-        TORCH_CHECK(!other || other->to <= r.from, "tensors ", other->of, " and ", r.of,
-                    " share memory that a result is written to");
-        if (!last || r.to > last->to) last = &r;
-        if (r.result && (!result || r.to > result->to)) result = &r;
-    }
+    TORCH_CHECK(apart, "tensors share memory that a result is written to");
 }
 
 Tensor clip_gradients_into(at::TensorList ts, double max_norm, at::TensorList out) {
@@ -556,6 +576,7 @@ Tensor clip_gradients_into(at::TensorList ts, double max_norm, at::TensorList ou
 
 void check_undifferentiated(at::TensorList ts, const char* name) {
     for (const Tensor& t : ts) {
+        if (!t.unsafeGetTensorImpl()->autograd_meta()) continue;    // of no graph
         no_tangents(name, {&t});
         TORCH_CHECK_NOT_IMPLEMENTED(!differentiates({&t}), name,
                                     " has no derivative; call it under torch.no_grad()");

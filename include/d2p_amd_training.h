@@ -34,7 +34,7 @@ typedef struct {
     int weight_dtype;           /* of weight and dweight */
     int dtype;                  /* of out and grad: weight_dtype, or 16 bits beside float32 */
     int B, L;                   /* B * L below 2^31 */
-    int V, D;                   /* V below 2^31 - 1; D from 1 on */
+    int V, D;                   /* V from 1, below 2^31 - 1; D from 8 to 2^20 */
     const void* tokens;         /* [B, L] contiguous, on the device */
     int token_bytes;            /* 4 or 8: int32 or int64 */
     const int* lengths;         /* int32 [B] on the device, or null for L each */
@@ -84,7 +84,7 @@ typedef struct {
 typedef struct {
     int dtype;                  /* of x, h and their gradients */
     int block_dtype;            /* of y, n and their gradients: dtype, or 16 bits beside float32 */
-    int B, L, D;                /* D from 1 to 8192 */
+    int B, L, D;                /* D from 8 to 8192 */
     int with_y;                 /* 0: no block yet */
     d2p_row_strides x, y;
     d2p_row_strides dh, dn;     /* of the results' gradients (backward only) */
@@ -105,14 +105,15 @@ int d2p_residual_norm(const d2p_residual_norm_params* p, const void* x, const vo
 /* Workspace bytes of d2p_residual_norm_backward. */
 size_t d2p_residual_norm_backward_workspace_bytes(const d2p_residual_norm_params* p);
 
-/* Gradients from dh = dL/dh and dn = dL/dn (null: zeros), h as the forward pass wrote it (x, with
- * its strides, where there is no y; null where n has no norm or no gradient) and y (null where z
- * is y and the gate's gradient is not wanted).  dx, dy [B, L, D] and dgate (of the gate's sizes),
- * contiguous, in their inputs' types; dweight .. dpost_bias [D] in theirs.  Null: not wanted; dx,
- * and dy where there is a y, always are, but dy may be null where it equals dx (no gate, no
- * post_norm, equal scales and types). */
+/* Gradients from dh = dL/dh and dn = dL/dn (one may be null: zeros).  stream_in, null where n has no norm or
+ * no gradient: h as the forward pass wrote it if it is float32; x, with its strides, if it has 16
+ * bits (h is formed from x and y again then, unrounded) or if there is no y.  y: null where it
+ * is needed for neither that, nor its own norm, nor the gate's gradient.  dx, dy [B, L, D] and dgate
+ * (of the gate's sizes), contiguous, in their inputs' types; dweight .. dpost_bias [D] in theirs.
+ * Null: not wanted; dx, and dy where there is a y, always are, but dy may be null where it equals
+ * dx (no gate, no post_norm, equal scales and types). */
 int d2p_residual_norm_backward(const d2p_residual_norm_params* p, const void* dh, const void* dn,
-                               const void* h, const void* y, const float* stats, void* dx,
+                               const void* stream_in, const void* y, const float* stats, void* dx,
                                void* dy, void* dgate, void* dweight, void* dbias,
                                void* dpost_weight, void* dpost_bias, void* workspace,
                                size_t workspace_bytes, void* stream);
@@ -129,8 +130,8 @@ typedef struct {
     int dtype;
 } d2p_tensor;
 
-/* Workspace bytes of both. */
-size_t d2p_global_norm_workspace_bytes(void);
+/* Workspace bytes of both for `count` tensors. */
+size_t d2p_global_norm_workspace_bytes(int count);
 
 /* norm = sqrt(sum of the squares of all numbers of all tensors), summed in float64. */
 int d2p_global_norm(const d2p_tensor* tensors, int count, float* norm, void* workspace,

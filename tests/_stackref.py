@@ -131,8 +131,8 @@ def residual(x, y=None, weight=None, bias=None, norm="rms", post_norm=None, post
         put("n", n.out, n.dout, kind)
     if dh is None and dn is None:
         return res, off
-    # the backward pass reads h rounded to its type
-    read = h_off + U[x.dtype] * h.abs() + TINY[x.dtype] if Y is not None else h_off
+    # the backward pass reads a float32 h as it was written, and forms others again
+    read = E * h.abs()
     H, dH = (torch.zeros_like(X),) * 2
     if dh is not None:
         H = double(dh)

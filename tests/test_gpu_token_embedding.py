@@ -53,7 +53,7 @@ def check(t, w, grad, lengths, scale=1.0, padding=None, dtype=None, dev="cuda"):
 CASES = [
     # V, B, L, D, weight, out, ragged, tokens' kind
     (5, 1, 1, 8, F32, F32, False, "mixed"),
-    (1, 2, 9, 1, F32, F32, False, "one"),
+    (1, 2, 9, 11, F32, F32, False, "one"),
     (21, 3, 50, 64, F32, BF16, True, "mixed"),
     (4, 7, 333, 40, BF16, BF16, True, "mixed"),
     (64, 2, 700, 512, F16, F16, False, "mixed"),
@@ -140,9 +140,6 @@ def test_shapes_strides_and_empty_calls(cuda):
         got = d2p_amd.token_embedding(torch.zeros(shape, dtype=torch.int64, device=cuda), wd)
         assert got.shape == (*shape, 24)
         assert not torch.autograd.grad(got.sum(), wd)[0].any()
-    none = torch.zeros(0, 24, device=cuda, requires_grad=True)
-    got = d2p_amd.token_embedding(t.to(cuda), none)
-    assert got.isnan().all() and torch.autograd.grad(got.sum(), none)[0].shape == (0, 24)
 
 
 def test_refusals(cuda):
@@ -150,7 +147,7 @@ def test_refusals(cuda):
     op = d2p_amd.token_embedding
     for call, match in (
             (lambda: op(t.float(), w), "int32 or int64"), (lambda: op(t, w.double()), "float32, float16"),
-            (lambda: op(t, w[0]), "2D"), (lambda: op(t, w[:, :0]), "features"),
+            (lambda: op(t, w[0]), "2D"), (lambda: op(t, w[:, :7]), "features"), (lambda: op(t, w[:0]), "rows"),
             (lambda: op(t, w.half(), dtype=torch.float32), "weight's type"),
             (lambda: op(t, w, torch.zeros(3, dtype=torch.int32, device=cuda)), "lengths must be"),
             (lambda: op(t, w, torch.zeros(2, dtype=torch.int64, device=cuda)), "lengths must be"),
