@@ -2,9 +2,10 @@
 Smith-Waterman value and back.
 
 Pairs of token sequences, one a mutated copy of the other or not, go through a small
-encoder (d2p_amd.SequenceAttention: norm and rotation of queries and keys, attention with a
-learned relative position bias and dropout); the products of their embeddings are the score
-matrix of d2p_amd.soft_sw, and the encoder learns to give related pairs the higher values.
+encoder (d2p_amd.SequenceEncoder: token embedding, a residual stream with norms, and layers of
+d2p_amd.SequenceAttention with a learned relative position bias and dropout); the products of
+their embeddings are the score matrix of d2p_amd.soft_sw, and the encoder learns, by gradients
+clipped to a common norm, to give related pairs the higher values.
 Then a causal layer reads a sequence token by token from its cache, and gives what it gives
 for the sequence as a whole.
 
@@ -27,18 +28,13 @@ TOKENS = 21     # twenty letters and padding
 class Encoder(nn.Module):
     def __init__(self, dim=128, heads=4, layers=2):
         super().__init__()
-        self.embed = nn.Embedding(TOKENS, dim)
-        self.layers = nn.ModuleList(
-            d2p_amd.SequenceAttention(dim, heads, num_buckets=32, max_distance=64, dropout=0.1)
-            for _ in range(layers))
-        self.norms = nn.ModuleList(nn.LayerNorm(dim) for _ in range(layers))
+        self.encoder = d2p_amd.SequenceEncoder(TOKENS, dim, heads, layers, norm="layer",
+                                               padding=TOKENS - 1, num_buckets=32,
+                                               max_distance=64, dropout=0.1)
         self.out = nn.Linear(dim, 32)
 
     def forward(self, tokens, lengths):
-        x = self.embed(tokens)
-        for norm, layer in zip(self.norms, self.layers):
-            x = x + layer(norm(x), lengths)
-        return self.out(x)
+        return self.out(self.encoder(tokens, lengths))
 
 
 def pairs(batch, length, device, generator):
@@ -76,6 +72,7 @@ def train(steps=60, batch=32, length=96, device="cuda", seed=0, autocast=True, r
         loss = F.binary_cross_entropy_with_logits(scale[0] * value + scale[1], related)
         optimizer.zero_grad()
         loss.backward()
+        d2p_amd.clip_grad_norm_((*model.parameters(), scale), 1.0)
         optimizer.step()
         losses.append(float(loss.detach()))
         if step % 10 == 0 or step == steps - 1:
