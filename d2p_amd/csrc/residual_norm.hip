@@ -454,14 +454,12 @@ int launch_backward(const ResidualBackArgs& a, int grid, hipStream_t st) {
 }
 
 // f(rows of whole runs, threads of a workgroup at most): rows within a wave, or of several
-template <class F> int by_row(int D, F f) {
-    using std::integral_constant;
-    const bool even = D % RUN == 0;
-    if (D <= 64 * RUN)
-        return even ? f(std::true_type{}, integral_constant<int, 256>{})
-                    : f(std::false_type{}, integral_constant<int, 256>{});
-    return even ? f(std::true_type{}, integral_constant<int, 1024>{})
-                : f(std::false_type{}, integral_constant<int, 1024>{});
+template <class F> int by_rows(int D, F f) {
+    const auto more = [&](auto most) {
+        return D % RUN ? f(std::false_type{}, most) : f(std::true_type{}, most);
+    };
+    return D <= 64 * RUN ? more(std::integral_constant<int, 256>{})
+                         : more(std::integral_constant<int, 1024>{});
 }
 
 // How the backward pass cuts rows into segments: at most as many as the card's 256 compute units
@@ -506,7 +504,7 @@ extern "C" int d2p_residual_norm(const d2p_residual_norm_params* p, const void* 
         using TX = typename decltype(tx)::type;
         using TY = typename decltype(ty)::type;
         const auto st = (hipStream_t)stream;
-        return by_row(p->D, [&](auto even, auto most) {
+        return by_rows(p->D, [&](auto even, auto most) {
             return y ? launch_forward<TX, TY, true, even(), most()>(a, grid, st)
                      : launch_forward<TX, TY, false, even(), most()>(a, grid, st);
         });
@@ -597,7 +595,7 @@ extern "C" int d2p_residual_norm_backward(const d2p_residual_norm_params* p, con
             using TX = typename decltype(tx)::type;
             using TY = typename decltype(ty)::type;
             const auto st = (hipStream_t)stream;
-            return by_row(p->D, [&](auto even, auto most) {
+            return by_rows(p->D, [&](auto even, auto most) {
                 return dy || again ? launch_backward<TX, TY, true, even(), most()>(a, cut.grid, st)
                                    : launch_backward<TX, TY, false, even(), most()>(a, cut.grid, st);
             });

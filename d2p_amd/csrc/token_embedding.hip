@@ -182,7 +182,9 @@ __device__ __forceinline__ void digit_bases(SortLds& s, const unsigned* counts, 
 // Lanes of the wave whose digit is this lane's, among the lanes that are `on`.
 __device__ __forceinline__ unsigned long long same_digit(unsigned digit, int bits, bool on) {
     unsigned long long m = __ballot(on);
-    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < MOST_BITS; ++b) {
+        if (b >= bits) break;
         const unsigned long long ones = __ballot(digit >> b & 1);
         m &= digit >> b & 1 ? ones : ~ones;
     }
@@ -197,10 +199,19 @@ __device__ __forceinline__ void place_keys(SortLds& s, int bits, const unsigned 
     const int lane = threadIdx.x & 63;
     unsigned* mine = s.wave + (threadIdx.x >> 6) * s.digits;
     for (int i = lane; i < s.digits; i += 64) mine[i] = 0;
-    __builtin_amdgcn_wave_barrier();
+    // places among the wave's keys.  (A wave's LDS accesses run in their order: all lanes have
+    // read before the first one of a digit writes)
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-        if (64 * i + lane < here) atomicAdd(&mine[digit[i]], 1u);
+    for (int i = 0; i < ITEMS; ++i) {
+        const bool on = 64 * i + lane < here;
+        const unsigned long long peers = same_digit(digit[i], bits, on);
+        const int rank = __popcll(peers & ((1ULL << lane) - 1));
+        __builtin_amdgcn_wave_barrier();
+        const unsigned before = on ? mine[digit[i]] : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (on && rank == 0) mine[digit[i]] = before + __popcll(peers);
+        place[i] = before + rank;
+    }
     __syncthreads();
     if ((int)threadIdx.x < s.digits) {
         unsigned next = s.base[threadIdx.x], c[SORT_WAVES];
@@ -215,16 +226,8 @@ __device__ __forceinline__ void place_keys(SortLds& s, int bits, const unsigned 
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        const bool on = 64 * i + lane < here;
-        const unsigned long long peers = same_digit(digit[i], bits, on);
-        const int rank = __popcll(peers & ((1ULL << lane) - 1));
-        place[i] = on ? mine[digit[i]] + rank : 0;
-        // (a wave's LDS accesses run in their order: all have read before the first one adds)
-        __builtin_amdgcn_wave_barrier();
-        if (on && rank == 0) atomicAdd(&mine[digit[i]], (unsigned)__popcll(peers));
-        __builtin_amdgcn_wave_barrier();
-    }
+    for (int i = 0; i < ITEMS; ++i)
+        if (64 * i + lane < here) place[i] += mine[digit[i]];
 }
 
 // Moves each key and its position to their places by the digit.  (Counting the next pass's digits
@@ -247,8 +250,8 @@ __global__ void __launch_bounds__(SORT_THREADS) move_keys_kernel(SortArgs a) {
             at[i] = k < here && !a.first ? a.at[n] : (unsigned)n;
             digit[i] = key[i] >> a.shift & (s.digits - 1);
         }
+        __syncthreads();        // (the part before has its places)
         if (part == n0) digit_bases(s, a.counts, a.tiles, blockIdx.x);
-        __syncthreads();
         place_keys(s, a.bits, digit, here, place);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
@@ -384,8 +387,8 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
             const bool on = i + u < i1 && k[u >> 2][u & 3] < V;
             const unsigned at = on ? n[u >> 2][u & 3] : 0;
             const unsigned b = a.by_length(at), l = at - b * p.L;
-            r[u] = load_run((const TO*)a.grad + (long long)b * p.grad.batch +
-                            (long long)l * p.grad.row, f, D);
+            r[u] = load_run<true>((const TO*)a.grad + (long long)b * p.grad.batch +
+                                  (long long)l * p.grad.row, f, D);
         }
         places(min(i + 8, i1 - 1 & ~7));
 #pragma unroll
