@@ -401,6 +401,9 @@ int check(const d2p_residual_norm_params* p) {
         D2P_REQUIRE(kind >= D2P_NORM_NONE && kind <= D2P_NORM_LAYER, "unknown norm");
     for (const d2p_vector* v : {&p->weight, &p->bias, &p->post_weight, &p->post_bias})
         D2P_TRY(check_vector(*v));
+    D2P_REQUIRE((p->norm != D2P_NORM_NONE || !(p->weight.data || p->bias.data)) &&
+                    (p->post_norm != D2P_NORM_NONE || !(p->post_weight.data || p->post_bias.data)),
+                "a norm's weight and bias need the norm");
     D2P_REQUIRE(p->gate_kind >= D2P_GATE_NONE && p->gate_kind <= D2P_GATE_TOKEN, "unknown gate");
     D2P_REQUIRE(p->gate_kind == D2P_GATE_NONE || p->gate_dtype == D2P_FLOAT32 ||
                     p->gate_dtype == p->block_dtype,

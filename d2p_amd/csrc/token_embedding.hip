@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
     }
     const int c = (blockIdx.x / a.slabs) * teams + team, f = blockIdx.x % a.slabs * SLAB + n0;
     if (c >= a.chunks || f >= D) return;
-    const int left = D - f, i0 = c * a.chunk, i1 = min(i0 + a.chunk, a.N);
+    const int left = D - f;
+    const unsigned N = a.N, i0 = c * a.chunk, i1 = min(i0 + a.chunk, N);   // (N + 8 may pass 2^31)
     unsigned run = i0 ? a.keys[i0 - 1] : V;     // the token before the chunk
     bool inside = false;                        // the run began in the chunk
     auto flush = [&](bool ended) {
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
     bool any = false;                           // acc holds a part of `run`
     // the next eight rows' places are under way with these eight rows
     u4v next[4];
-    auto places = [&](int i) {
+    auto places = [&](unsigned i) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             next[q] = *(const u4v*)(a.keys + i + 4 * q);
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
         }
     };
     places(i0);
-    for (int i = i0; i < i1; i += 8) {
+    for (unsigned i = i0; i < i1; i += 8) {
         const u4v k[2] = {next[0], next[1]}, n[2] = {next[2], next[3]};
         if (k[0][0] >= V) break;                // only unused positions are left
         Eight<TO> r[8];
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
             r[u] = load_run<true>((const TO*)a.grad + (long long)b * p.grad.batch +
                                   (long long)l * p.grad.row, f, D);
         }
-        places(min(i + 8, i1 - 1 & ~7));
+        places(min(i + 8, i1 - 1 & ~7u));
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             if (i + u >= i1) break;
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
             for (int e = 0; e < RUN; ++e) acc[e] += x[e];
         }
     }
-    if (any) flush(i1 >= a.N || a.keys[i1] != run);
+    if (any) flush(i1 >= N || a.keys[i1] != run);
 }
 
 // Joins the parts of each run that begins in chunk c and ends in a later one: the waves of a
@@ -419,8 +420,8 @@ __global__ void __launch_bounds__(256) join_runs_kernel(TableArgs a) {
     __shared__ float part[4][SLAB];
     const int D = a.p.D, c = blockIdx.x / a.slabs, f0 = blockIdx.x % a.slabs * SLAB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = c * a.chunk, i1 = i0 + a.chunk;
-    if (i1 >= a.N) return;
+    const unsigned i0 = c * a.chunk, i1 = i0 + a.chunk;
+    if (i1 >= (unsigned)a.N) return;
     const unsigned run = a.keys[i1 - 1];
     if (run >= (unsigned)a.p.V || a.keys[i1] != run) return;            // none goes on
     if (a.keys[i0] == run && i0 && a.keys[i0 - 1] == run) return;      // it began earlier
@@ -489,13 +490,13 @@ template <class TO> __global__ void __launch_bounds__(256) table_grad_small_kern
     const int split = blockIdx.x / a.slabs;
     const int f = blockIdx.x % a.slabs * SLAB + (me & (a.lanes - 1)) * 2;
     const long long N = (long long)p.B * p.L;
-    const int r0 = min((long long)split * a.rows, N), r1 = min((long long)r0 + a.rows, N);
+    const unsigned r0 = min((long long)split * a.rows, N), r1 = min((long long)r0 + a.rows, N);
     // behind the features' end the last two are read; of a lone last one, it and the one before
     const int f0 = min(f, p.D - 2);
     const bool lone = f == p.D - 1;
     for (int i = 0; i < p.V * 2; ++i) sums[i * 256 + me] = 0.0f;
-    for (int part = r0; part < r1; part += SMALL_ROWS) {
-        const int rows = min(SMALL_ROWS, r1 - part);
+    for (unsigned part = r0; part < r1; part += SMALL_ROWS) {
+        const int rows = min(SMALL_ROWS, (int)(r1 - part));
         __syncthreads();
         for (int i = me; i < rows; i += 256) tokens[i] = token_at(p, a.by_length, part + i);
         __syncthreads();
@@ -730,7 +731,7 @@ extern "C" int d2p_token_embedding_backward(const d2p_token_embedding_params* p,
     a.head = (float*)(ws + plan.total - 2 * plan.parts);
     a.tail = (float*)(ws + plan.total - plan.parts);
     const int teams = 256 / plan.lanes;
-    D2P_REQUIRE((long long)plan.chunks * plan.slabs < 1LL << 30, "too many tokens and features");
+    D2P_REQUIRE((long long)plan.chunks * plan.slabs < 1LL << 24, "too many tokens and features");
     a.sum_blocks = cdiv(plan.chunks, teams) * plan.slabs;
     a.zero_blocks = std::min(cdiv(p->V, teams), 4 * std::max(device_cus(), 1));
     D2P_TRY(launch_sort(*p, plan, ws, a, st));

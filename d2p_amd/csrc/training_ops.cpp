@@ -45,7 +45,6 @@ EmbedInputs embed_inputs(const Tensor& tokens, const OptTensor& lengths, double 
     TORCH_CHECK(tokens.is_cuda(), "tokens must be a CUDA tensor");
     TORCH_CHECK(tokens.scalar_type() == torch::kInt32 || tokens.scalar_type() == torch::kInt64,
                 "tokens must be int32 or int64, got ", tokens.scalar_type());
-    in.tokens = tokens.contiguous();
     const bool batched = tokens.dim() == 2;
     p.B = batched ? dim32(tokens.size(0), "batch size") : 1;
     p.L = dim32(batched ? tokens.size(1) : tokens.numel(), "length");
@@ -59,6 +58,7 @@ EmbedInputs embed_inputs(const Tensor& tokens, const OptTensor& lengths, double 
     p.dtype = dtype;
     TORCH_CHECK(weight_dtype == dtype || weight_dtype == D2P_FLOAT32,
                 "embeddings must be of the weight's type, or of 16 bits beside a float32 weight");
+    in.tokens = tokens.contiguous();
     p.tokens = in.tokens.data_ptr();
     p.token_bytes = (int)tokens.element_size();
     if (given(lengths)) {

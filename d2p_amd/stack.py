@@ -126,11 +126,10 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]],
     """Clips the gradients of ``parameters`` in place to a common 2-norm of ``max_norm`` at most,
     and returns the norm that they had (float32, on the device).  Parameters without a gradient
     are left out, one that is listed twice counts once."""
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = {id(p.grad): p.grad for p in parameters if p.grad is not None}
     if not grads:
-        return torch.zeros(())
+        return torch.zeros((), device=parameters[0].device if parameters else None)
     grads = list(grads.values())
     return torch.ops.d2p_amd.clip_gradients_into(grads, float(max_norm), grads)
 

@@ -140,6 +140,8 @@ def test_embedding_pointers_and_workspaces(lib):
     (dict(B=1 << 20, L=1 << 11), "too many"), (dict(D=7), "features"), (dict(D=8193), "features"),
     (dict(norm=3), "norm"), (dict(post_norm=-1), "norm"), (dict(weight=Vector(0x1000, 7)), "vector"),
     (dict(post_bias=Vector(0x1000, -1)), "vector"), (dict(gate_kind=4), "gate"),
+    (dict(norm=0, weight=Vector(0x1000, 0)), "need the norm"),
+    (dict(post_bias=Vector(0x1000, 0)), "need the norm"),
     (dict(gate_kind=1, gate=FAKE, gate_dtype=1), "gate must"), (dict(gate_kind=2), "null"),
     (dict(eps=-1.0), "eps"), (dict(eps=NAN), "eps")], ids=str)
 def test_residual_checks(lib, kw, match):
@@ -252,6 +254,14 @@ def test_python_layer_checks():
         with pytest.raises(ValueError, match=match):
             call()
     assert float(d2p_amd.clip_grad_norm_([v], 1.0)) == 0.0        # no gradient at all
+
+
+def test_clipping_nothing_gives_zero_where_the_parameters_are():
+    for device in ("cpu", "meta"):
+        p = torch.nn.Parameter(torch.zeros(3, device=device))
+        norm = d2p_amd.clip_grad_norm_(iter([p]), 1.0)
+        assert norm.device == p.device and norm.shape == () and norm.dtype == torch.float32
+    assert float(d2p_amd.clip_grad_norm_([], 1.0)) == 0.0
 
 
 def test_encoder_parameters():
