@@ -270,11 +270,11 @@ residual_norm_backward_kernel(ResidualBackArgs a) {
             Eight<TY> ry;
             GateRun<TY, EVEN> rg;
             f4v st = *(const f4v*)(a.stats + a.stats_step * min(row, r1 - 1));
-            const Eight<TX> rdh = load_run(place.in<TX>(a.dh, p.dh), vat, D);
-            const Eight<TY> rdn = load_run(place.in<TY>(a.dn, p.dn), vat, D);
-            const Eight<TX> rs = load_run(place.in<TX>(a.stream, p.x), vat, D);
+            const Eight<TX> rdh = load_run<true>(place.in<TX>(a.dh, p.dh), vat, D);
+            const Eight<TY> rdn = load_run<true>(place.in<TY>(a.dn, p.dn), vat, D);
+            const Eight<TX> rs = load_run<true>(place.in<TX>(a.stream, p.x), vat, D);
             if (BLOCK) {
-                ry = load_run(place.in<TY>(a.y, p.y), vat, D);
+                ry = load_run<true>(place.in<TY>(a.y, p.y), vat, D);
                 if (by_row) rg.load(place);
             }
             const bool there = row < r1;

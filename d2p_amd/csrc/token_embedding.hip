@@ -10,6 +10,7 @@
 // last kernel joins those.  Tokens that do not occur are marked by the sort's last pass, and
 // their rows zeroed beside the sums, so that every row is written once.
 #include <algorithm>
+#include <type_traits>
 
 #include "training.hip.h"
 
@@ -182,9 +183,7 @@ __device__ __forceinline__ void digit_bases(SortLds& s, const unsigned* counts, 
 // Lanes of the wave whose digit is this lane's, among the lanes that are `on`.
 __device__ __forceinline__ unsigned long long same_digit(unsigned digit, int bits, bool on) {
     unsigned long long m = __ballot(on);
-#pragma unroll
-    for (int b = 0; b < MOST_BITS; ++b) {
-        if (b >= bits) break;
+    for (int b = 0; b < bits; ++b) {
         const unsigned long long ones = __ballot(digit >> b & 1);
         m &= digit >> b & 1 ? ones : ~ones;
     }
@@ -264,28 +263,29 @@ __global__ void __launch_bounds__(SORT_THREADS) move_keys_kernel(SortArgs a) {
 }
 
 // All of a short sort in one workgroup: the passes exchange through LDS.
-constexpr int SHORT_ITEMS = 8, SHORT = SORT_THREADS * SHORT_ITEMS;
+template <int ITEMS>
 __global__ void __launch_bounds__(SORT_THREADS) sort_short_kernel(SortArgs a, int passes) {
+    constexpr int MOST = SORT_THREADS * ITEMS;
     extern __shared__ unsigned sort_lds[];
-    SortLds s(sort_lds + 2 * SHORT, a.bits);
-    unsigned *keys = sort_lds, *ats = sort_lds + SHORT;
+    SortLds s(sort_lds + 2 * MOST, a.bits);
+    unsigned *keys = sort_lds, *ats = sort_lds + MOST;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int w0 = wave * 64 * SHORT_ITEMS;
-    const int here = min(max(a.N - w0, 0), 64 * SHORT_ITEMS);
+    const int w0 = wave * 64 * ITEMS;
+    const int here = min(max(a.N - w0, 0), 64 * ITEMS);
     clear_present(a, threadIdx.x, SORT_THREADS);
-    unsigned key[SHORT_ITEMS], at[SHORT_ITEMS];
+    unsigned key[ITEMS], at[ITEMS];
 #pragma unroll
-    for (int i = 0; i < SHORT_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         const int n = w0 + 64 * i + lane;
         key[i] = n < a.N ? key_at(a, n) : 0;
         at[i] = n;
     }
     for (int pass = 0; pass < passes; ++pass) {
-        unsigned digit[SHORT_ITEMS], place[SHORT_ITEMS];
+        unsigned digit[ITEMS], place[ITEMS];
         s.part[threadIdx.x] = 0;        // (one tile, whose counts lie here)
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < SHORT_ITEMS; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             digit[i] = key[i] >> (pass * a.bits) & (s.digits - 1);
             if (64 * i + lane < here) atomicAdd(&s.part[digit[i]], 1u);
         }
@@ -294,14 +294,14 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_short_kernel(SortArgs a, in
         __syncthreads();
         place_keys(s, a.bits, digit, here, place);
 #pragma unroll
-        for (int i = 0; i < SHORT_ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i)
             if (64 * i + lane < here) {
                 keys[place[i]] = key[i];
                 ats[place[i]] = at[i];
             }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < SHORT_ITEMS; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             const int n = w0 + 64 * i + lane;
             key[i] = n < a.N ? keys[n] : 0;
             at[i] = n < a.N ? ats[n] : 0;
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_short_kernel(SortArgs a, in
         __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < SHORT_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
         const int n = w0 + 64 * i + lane;
         if (n >= a.N) continue;
         a.keys_to[n] = key[i];
@@ -555,7 +555,13 @@ int check(const d2p_token_embedding_params* p) {
 
 size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-constexpr int SMALL = 32;
+// Up to here one workgroup sorts all keys.  bf16 [N, 256], V 4097, the whole gradient: N 64 11.4 us
+// (by tiles 18.6), 1024 15.0 (22.6), 4096 21.9 (27.7); 8192 keys 31.8 (29.9).
+constexpr int SHORT = 4 * SORT_THREADS;
+// A table of up to SMALL tokens and SMALL_TABLE numbers needs no sort.  bf16, 16384 rows: V 21, D 256
+// 13.6 us (24.7 sorted), V 21, D 512 19.6 (22.0), V 64, D 64 about 15 (28); V 32, D 512 20.8 (21.2)
+// and with 131072 rows 51.7 (47.0), V 64, D 256 22.0 (20.5), V 21, D 2048 33.7 (30.5).
+constexpr int SMALL = 64, SMALL_TABLE = 12288;
 
 // How the backward pass splits its work, and its workspace.
 struct Plan {
@@ -578,7 +584,7 @@ struct Plan {
         lanes = std::min(team_of(p.D), 64);
         slabs = cdiv(p.D, SLAB);
         splits = 0;
-        if (p.V <= SMALL && (long long)p.V * p.D <= 1 << 24) {
+        if (p.V <= SMALL && (long long)p.V * p.D <= SMALL_TABLE) {
             // workgroups that the card's LDS holds at a time, each with more rows than its table has
             const int groups = 256 * std::min(8, 156 / (2 * p.V));
             splits = std::max(1, std::min(groups / slabs, N / (2 * p.V)));
@@ -587,11 +593,16 @@ struct Plan {
             total = (size_t)splits * p.V * p.D * 4;
             return;
         }
-        // chunks of 64 positions where they give the card's waves work, shorter ones where
-        // positions are few, longer ones where the joins of long runs would be
+        // As many waves as the card has SIMDs, of chunks from 8 to 128 positions; longer ones where
+        // that leaves very many.  bf16, us with 16, 32, 64, 128, 256 positions (* taken):
+        //   N 16384,   V 4097,  D 512:    33*  35   42   56   85   (8: 36)
+        //   N 131072,  V 65536, D 64:     48*  49   56   74  112   (8: 54)
+        //   N 131072,  V 200,   D 1024:  124   95   77   67*  73
+        //   N 131072,  V 65536, D 1024:  120  112  107  107* 121
+        //   N 4194304, V 65536, D 64:    592  482  419  390* 379
         const long long waves = (long long)N * slabs * lanes / 64;
         chunk = 8;
-        while (chunk < 256 && waves / chunk > 4096) chunk *= 2;
+        while (chunk < (waves / chunk >= 1 << 16 ? 256 : 128) && waves / chunk > 1024) chunk *= 2;
         chunks = cdiv(N, chunk);
         keys = round16(((size_t)N + 8) * 4);
         counts = round16(((size_t)tiles << bits) * 4);
@@ -644,11 +655,18 @@ int launch_sort(const d2p_token_embedding_params& p, const Plan& plan, char* ws,
     a.present = (unsigned char*)(ws + 4 * plan.keys + plan.counts);
     t.present = a.present;
     if (plan.short_sort) {
-        static LdsAllowed known;
-        D2P_TRY(allow_lds((const void*)sort_short_kernel, known));
-        D2P_LAUNCH("token_sort", sort_short_kernel, dim3(1), dim3(SORT_THREADS),
-                   2 * SHORT * sizeof(unsigned) + SortLds::bytes(plan.bits), st, a, plan.passes);
-        D2P_HIP(hipGetLastError());
+        const auto sort = [&](auto items) {
+            static LdsAllowed known;
+            D2P_TRY(allow_lds((const void*)sort_short_kernel<items()>, known));
+            D2P_LAUNCH("token_sort", sort_short_kernel<items()>, dim3(1), dim3(SORT_THREADS),
+                       2 * SORT_THREADS * items() * sizeof(unsigned) + SortLds::bytes(plan.bits), st,
+                       a, plan.passes);
+            D2P_HIP(hipGetLastError());
+            return D2P_OK;
+        };
+        D2P_TRY(plan.N <= SORT_THREADS       ? sort(std::integral_constant<int, 1>{})
+                : plan.N <= 2 * SORT_THREADS ? sort(std::integral_constant<int, 2>{})
+                                             : sort(std::integral_constant<int, 4>{}));
     }
     for (int n = 0; n < plan.passes && !plan.short_sort; ++n) {
         a.first = n == 0;

@@ -45,18 +45,15 @@ template <class T> __device__ __forceinline__ Eight<T> to_front(const Eight<T>& 
 // row whatever `at` is, at the row's end the last eight, which unpack then moves into place.
 // (A branch around each load, and its conversion behind it, made the loads wait for each other.)
 //
-// PAST: past the caches, for what is read once (gradients into a table's sums: [16, 8192, 1024] of
-// 65536 bfloat16, 102 -> 82 us).
+// PAST: past the caches, for what is read once.  Of 16-bit numbers only: float32 takes two loads
+// a lane, each of half a line, which then comes twice.
 typedef u4v u4v_any __attribute__((aligned(2)));
 template <bool PAST = false, class T>
 __device__ __forceinline__ Eight<T> load_run(const T* row, int at, int D) {
     const T* p = row + min(at, D - RUN);
-    if (!PAST) return *(const Eight<T>*)p;
-    struct Chunks { u4v v[sizeof(T) / 2]; } r;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        r.v[i] = __builtin_nontemporal_load((const u4v_any*)p + i);
-    return bits<Eight<T>>(r);
+    if constexpr (PAST && sizeof(T) == 2)
+        return bits<Eight<T>>(__builtin_nontemporal_load((const u4v_any*)p));
+    return *(const Eight<T>*)p;
 }
 // x = the numbers; zeros behind the row's end, and where the row is not wanted.  EVEN: D is known to
 // be a multiple of eight.

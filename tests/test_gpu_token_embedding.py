@@ -70,6 +70,19 @@ CASES = [
     (500, 1, 30011, 200, F16, F16, False, "pairs"),
     (12, 2, 4096, 1100, F32, F32, True, "mixed"),
     (2, 1, 3, 2000, F32, BF16, False, "mixed"),
+    # where one way of summing ends and the next begins
+    (64, 3, 900, 192, BF16, BF16, True, "mixed"),
+    (64, 3, 900, 193, BF16, BF16, True, "mixed"),
+    (33, 2, 50, 9, F32, F16, False, "mixed"),
+    (1, 1, 2000, 8, F16, F16, False, "mixed"),
+    (1, 1, 700, 12289, F32, F32, False, "mixed"),
+    (3000, 1, 1024, 40, BF16, BF16, False, "pairs"),
+    (3000, 1, 1025, 40, BF16, BF16, False, "pairs"),
+    (200, 1, 2048, 40, F32, F32, False, "falling"),
+    (200, 1, 2049, 40, F32, F32, False, "falling"),
+    (70000, 2, 2048, 16, F16, F16, True, "mixed"),
+    (70000, 1, 4097, 16, F16, F16, False, "mixed"),
+    (1100000, 1, 3000, 8, F32, F32, False, "mixed"),
 ]
 
 
