@@ -413,13 +413,13 @@ __global__ void __launch_bounds__(256) table_grad_kernel(TableArgs a) {
     if (any) flush(i1 >= N || a.keys[i1] != run);
 }
 
-// Joins the parts of each run that begins in chunk c and ends in a later one: the waves of a
+// Joins the parts of each run that begins in chunk c and ends in a later one: the teams of a
 // workgroup take them in turn, four at a time, and their sums meet in order.
 template <class TW>
 __global__ void __launch_bounds__(256) join_runs_kernel(TableArgs a) {
-    __shared__ float part[4][SLAB];
+    __shared__ __align__(16) float part[256 * RUN];
     const int D = a.p.D, c = blockIdx.x / a.slabs, f0 = blockIdx.x % a.slabs * SLAB;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, team = threadIdx.x / a.lanes, teams = 256 / a.lanes;
     const unsigned i0 = c * a.chunk, i1 = i0 + a.chunk;
     if (i1 >= (unsigned)a.N) return;
     const unsigned run = a.keys[i1 - 1];
@@ -436,33 +436,32 @@ __global__ void __launch_bounds__(256) join_runs_kernel(TableArgs a) {
         }
         last += 64;
     }
-    const int f = f0 + lane * RUN, left = D - f;
+    const int f = f0 + (threadIdx.x & (a.lanes - 1)) * RUN;
     float acc[RUN] = {};
-    if (wave == 0) unpack(load_run(a.tail + (long long)c * D, f, D), f, D, true, acc);
-    for (int k = c + 1 + wave; k <= last; k += 16) {
+    if (team == 0) unpack(load_run(a.tail + (long long)c * D, f, D), f, D, true, acc);
+    for (int k = c + 1 + team; k <= last; k += 4 * teams) {
         Eight<float> r[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) r[u] = load_run(a.head + (long long)min(k + 4 * u, last) * D, f, D);
+        for (int u = 0; u < 4; ++u)
+            r[u] = load_run(a.head + (long long)min(k + teams * u, last) * D, f, D);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             float x[RUN];
-            unpack(r[u], f, D, k + 4 * u <= last, x);
+            unpack(r[u], f, D, k + teams * u <= last, x);
 #pragma unroll
             for (int e = 0; e < RUN; ++e) acc[e] += x[e];
         }
     }
-#pragma unroll
-    for (int e = 0; e < RUN; ++e) part[wave][64 * e + lane] = acc[e];
+    f4v* mine = (f4v*)(part + threadIdx.x * RUN);
+    mine[0] = f4v{acc[0], acc[1], acc[2], acc[3]};
+    mine[1] = f4v{acc[4], acc[5], acc[6], acc[7]};
     __syncthreads();
-    if (wave) return;
-#pragma unroll
-    for (int e = 0; e < RUN; ++e) {
+    const int numbers = a.lanes * RUN;
+    for (int d = threadIdx.x; d < min(numbers, D - f0); d += 256) {
         float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) s += part[w][64 * e + lane];
-        acc[e] = s * a.p.scale;
+        for (int t = 0; t < teams; ++t) s += part[t * numbers + d];
+        ((TW*)a.dweight)[(long long)run * D + f0 + d] = (TW)(s * a.p.scale);
     }
-    store_run((TW*)a.dweight + (long long)run * D + f, left, acc);
 }
 
 // ---------------------------------------------------------------------------
