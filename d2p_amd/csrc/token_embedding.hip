@@ -1,7 +1,10 @@
 // token_embedding.hip -- rows of a table by token, and the table's gradient
 // (include/d2p_amd_training.h).
 //
-// Forward: bound by writing the result; a team of lanes copies rows, eight numbers a lane.
+// Forward: bound by reading rows and writing the result; a team of lanes copies rows, eight
+// numbers a lane, four rows in flight (two: 42 us for 38 at [262144, 256] of 30000, eight 44), in
+// eight workgroups a compute unit (as many as there are rows: 67).  bf16 [131072, 1024] of 65536 tokens
+// in 80 us: 3.4 TB/s written, about 5 with what is read.
 //
 // Backward: the gradient's rows of one token have to come together.  Positions are sorted by
 // token (a stable radix sort of up to ten bits a pass, so that sums have one order), cut into chunks
@@ -27,6 +30,10 @@ struct EmbedArgs {
     Divisor by_length;
 };
 constexpr int DEEP = 4;             // rows that a team has in flight
+// As much as the card's last cache holds is written past it: bf16 [131072, 1024] of 65536 tokens 80
+// us, 103 without; with the norm that reads it next 201 either way.  Less is left for that norm:
+// [65536, 512] 42.4 us, 44.2 past the caches.
+constexpr long long CACHES = 256 << 20;
 
 // The token at position n of [B, L]: its row; ABSENT for padding and past its sequence's
 // length; WRONG for one that the table does not have or whose sequence's length is out of range.
@@ -44,7 +51,8 @@ __device__ __forceinline__ int token_at(const d2p_token_embedding_params& p,
     return t >= 0 && t < p.V ? (int)t : WRONG;
 }
 
-template <class TW, class TO>
+// PAST: more is written than any cache keeps
+template <class TW, class TO, bool PAST>
 __global__ void __launch_bounds__(256) token_embedding_kernel(EmbedArgs a) {
     const d2p_token_embedding_params& p = a.p;
     const int n0 = threadIdx.x & (a.lanes - 1), teams = 256 / a.lanes;
@@ -67,7 +75,7 @@ __global__ void __launch_bounds__(256) token_embedding_kernel(EmbedArgs a) {
 #pragma unroll
                 for (int e = 0; e < RUN; ++e) x[e] = t[u] == WRONG ? __builtin_nanf("") : x[e] * p.scale;
                 if (row + u * step < rows)
-                    store_run((TO*)a.out + (row + u * step) * p.D + at, p.D - at, x);
+                    store_run<PAST>((TO*)a.out + (row + u * step) * p.D + at, p.D - at, x);
             }
         }
     }
@@ -558,8 +566,8 @@ size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 // (by tiles 18.6), 1024 15.0 (22.6), 4096 21.9 (27.7); 8192 keys 31.8 (29.9).
 constexpr int SHORT = 4 * SORT_THREADS;
 // A table of up to SMALL tokens and SMALL_TABLE numbers needs no sort.  bf16, 16384 rows: V 21, D 256
-// 13.6 us (24.7 sorted), V 21, D 512 19.6 (22.0), V 64, D 64 about 15 (28); V 32, D 512 20.8 (21.2)
-// and with 131072 rows 51.7 (47.0), V 64, D 256 22.0 (20.5), V 21, D 2048 33.7 (30.5).
+// 13.5 us (21.5 sorted), V 21, D 512 19.0 (22.2), V 64, D 64 11.7 (18.3); above, V 32, D 512 20.8
+// (21.3) and with 131072 rows 51.7 (47.4), V 64, D 256 22.2 (19.0).
 constexpr int SMALL = 64, SMALL_TABLE = 12288;
 
 // How the backward pass splits its work, and its workspace.
@@ -708,8 +716,10 @@ extern "C" int d2p_token_embedding(const d2p_token_embedding_params* p, const vo
     return with_pair(p->weight_dtype, p->dtype, [&](auto tw, auto to) {
         using TW = typename decltype(tw)::type;
         using TO = typename decltype(to)::type;
-        D2P_LAUNCH("token_embedding", (token_embedding_kernel<TW, TO>), dim3(grid), dim3(256), 0,
-                   (hipStream_t)stream, a);
+        const bool past = (long long)p->B * p->L * p->D * (int)sizeof(TO) >= CACHES;
+        const auto kernel = past ? token_embedding_kernel<TW, TO, true>
+                                 : token_embedding_kernel<TW, TO, false>;
+        D2P_LAUNCH("token_embedding", kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, a);
         D2P_HIP(hipGetLastError());
         return D2P_OK;
     });

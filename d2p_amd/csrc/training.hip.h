@@ -69,12 +69,16 @@ __device__ __forceinline__ void unpack(const Eight<T>& a, int at, int D, bool wa
 template <class T, int N> struct Few {
     T v[N];
 };
-template <class T> __device__ __forceinline__ void store_run(T* p, int left, const float* x) {
+template <bool PAST = false, class T>
+__device__ __forceinline__ void store_run(T* p, int left, const float* x) {
     Eight<T> a;
 #pragma unroll
     for (int e = 0; e < RUN; ++e) a.v[e] = (T)x[e];
     if (left >= RUN) {
-        *(Eight<T>*)p = a;
+        if constexpr (PAST && sizeof(T) == 2)
+            __builtin_nontemporal_store(bits<u4v>(a), (u4v_any*)p);
+        else
+            *(Eight<T>*)p = a;
     } else if (left > 0) {      // four, two and one
         const bool four = left & 4, two = left & 2;
         if (four) *(Few<T, 4>*)p = {a.v[0], a.v[1], a.v[2], a.v[3]};
