@@ -585,7 +585,10 @@ struct Plan {
         passes = cdiv(bits, MOST_BITS);
         bits = cdiv(bits, passes);
         short_sort = N <= SHORT && p.V <= 1 << 20;
-        tile_bits = 11;         // two keys a thread
+        // tiles of one key a thread, and where those would be too many for each to add up all
+        // counts, of two and more (bf16, V 65536: [32768, 64] 31.7 us, 37.9 with two a thread;
+        // [1048576, 64] 133.8, 138.8 with one)
+        tile_bits = N <= MOST_TILES * SORT_THREADS ? 10 : 11;
         while (cdiv(N, 1 << tile_bits) > MOST_TILES) ++tile_bits;
         tiles = std::max(1, cdiv(N, 1 << tile_bits));
         lanes = std::min(team_of(p.D), 64);
@@ -687,11 +690,16 @@ int launch_sort(const d2p_token_embedding_params& p, const Plan& plan, char* ws,
         D2P_LAUNCH("token_sort_count", count_digits_kernel, dim3(std::max(plan.tiles, clearing)),
                    dim3(SORT_THREADS), 0, st, a);
         D2P_HIP(hipGetLastError());
-        static LdsAllowed known;
-        D2P_TRY(allow_lds((const void*)move_keys_kernel<2>, known));
-        D2P_LAUNCH("token_sort_move", move_keys_kernel<2>, dim3(plan.tiles), dim3(SORT_THREADS),
-                   SortLds::bytes(plan.bits), st, a);
-        D2P_HIP(hipGetLastError());
+        const auto move = [&](auto items) {
+            static LdsAllowed known;
+            D2P_TRY(allow_lds((const void*)move_keys_kernel<items()>, known));
+            D2P_LAUNCH("token_sort_move", move_keys_kernel<items()>, dim3(plan.tiles),
+                       dim3(SORT_THREADS), SortLds::bytes(plan.bits), st, a);
+            D2P_HIP(hipGetLastError());
+            return D2P_OK;
+        };
+        D2P_TRY(plan.tile_bits == 10 ? move(std::integral_constant<int, 1>{})
+                                     : move(std::integral_constant<int, 2>{}));
     }
     t.keys = a.keys_to;
     t.at = a.at_to;

@@ -83,6 +83,9 @@ CASES = [
     (70000, 2, 2048, 16, F16, F16, True, "mixed"),
     (70000, 1, 4097, 16, F16, F16, False, "mixed"),
     (1100000, 1, 3000, 8, F32, F32, False, "mixed"),
+    (5000, 1, 131072, 8, F32, F32, False, "mixed"),
+    (5000, 1, 131073, 8, F32, F32, False, "falling"),
+    (700, 3, 100001, 8, BF16, BF16, True, "pairs"),
 ]
 
 
