@@ -6,8 +6,13 @@
 // pointers; longer lists take several launches.  They leave the list in the workspace for the
 // second pass, which is one launch.  Tensors are cut into pieces of PIECE numbers; a workgroup
 // takes neighbouring ones, so that it looks its tensor up once, and takes them in falling order
-// in the second pass, which so begins with what the first one has left in the caches.  Squares
-// are summed in float64: no gradient's overflows it, and the vector units have the time.
+// in the second pass, which so begins with what the first one has left in the caches (320 M bf16:
+// 383 us in rising order, 367 in falling).  Squares are summed in float64: no gradient's
+// overflows it, and the vector units have the time.
+//
+// 320 M bf16 in 40 tensors: the norm in 113 us, 5.7 TB/s (a read alone reaches 6.1), clipping in 371
+// for both passes, 5.2 TB/s.  24 M numbers of three types in 301 tensors: 11 us for each of two lists,
+// 27 for the scaling.  280 k in 18 tensors: 6.5 and 5.5 us, most of it launches and the lookup.
 #include <algorithm>
 
 #include "training.hip.h"
