@@ -241,10 +241,19 @@ __device__ __forceinline__ void flush(float* lds, const float* sums, float* dst,
     }
 }
 
+// Waves a SIMD that the backward pass's registers are held to: four, but three where h is formed
+// again and the biases' sums are kept too (in workgroups of 256 threads; larger ones keep a few
+// registers in scratch).  As many workgroups as that leaves room for: fp16 [5, 1023, 333], layer norms
+// and a gate by token, kernel 30 -> 20 us; bf16 [131072, 512], layer and RMS norm, 200 -> 165.
+constexpr int BACK_WAVES = 4;
+__host__ __device__ constexpr int back_waves(bool again, bool biases, int threads) {
+    return again && biases && threads == 256 ? 3 : BACK_WAVES;
+}
+
 // BLOCK: y has a gradient of its own (or, in 16 bits, h is formed from it again); BIASES: some
 // bias wants its gradient
 template <class TX, class TY, bool BLOCK, bool BIASES, bool EVEN, int MOST>
-__global__ void __launch_bounds__(MOST, BIASES && MOST == 256 ? 3 : 4)
+__global__ void __launch_bounds__(MOST, back_waves(BLOCK && sizeof(TX) == 2, BIASES, MOST))
 residual_norm_backward_kernel(ResidualBackArgs a) {
     constexpr bool WIDE = MOST > 256, AGAIN = BLOCK && sizeof(TX) == 2;
     // the teams' slots; the vectors; then, for the teams' sums, eight numbers a thread
@@ -483,18 +492,20 @@ template <class F> int by_rows(int D, F f) {
 }
 
 // How the backward pass cuts rows into segments: at most as many as the card's 256 compute units
-// hold at four waves a SIMD, no fewer while there are rows for it, and each of one sequence
+// hold at `waves` waves a SIMD, no fewer while there are rows for it, and each of one sequence
 // where the gate's gradient is by sequence.
 struct Cut {
     int batches, length, splits, grid;
-    Cut(const d2p_residual_norm_params& p, int lanes) {
+    Cut(const d2p_residual_norm_params& p, int lanes, int waves) {
         const int teams = threads_of(lanes) / lanes;
         const bool by_sequence = p.gate_kind == D2P_GATE_SEQUENCE;
         batches = by_sequence ? p.B : 1;
         length = by_sequence ? p.L : p.B * p.L;
-        const int groups = 256 * 1024 / threads_of(lanes);
+        const int groups = 256 * 256 * waves / threads_of(lanes);
         const int most = std::max(1, groups / std::max(batches, 1));
-        splits = std::min(most, std::max(1, cdiv(length, teams)));
+        // (whole turns of a workgroup's teams: float32 beside bf16 [5, 1023, 333], layer norms, 640
+        // workgroups of 8 rows 24 us, 1024 of 5 rows 29)
+        splits = std::max(1, cdiv(length, std::max(1, cdiv(cdiv(length, most), teams) * teams)));
         grid = (int)std::min<long long>((long long)batches * splits, groups);
     }
 };
@@ -534,7 +545,7 @@ extern "C" int d2p_residual_norm(const d2p_residual_norm_params* p, const void* 
 extern "C" size_t d2p_residual_norm_backward_workspace_bytes(const d2p_residual_norm_params* p) {
     if (!p || p->B < 0 || p->L < 0 || p->D < RUN || p->D > 8192 || (long long)p->B * p->L >= 1LL << 31)
         return 0;
-    const Cut cut(*p, team_of(p->D));
+    const Cut cut(*p, team_of(p->D), BACK_WAVES);
     const size_t gate = p->gate_kind == D2P_GATE_FEATURE || p->gate_kind == D2P_GATE_SEQUENCE
                             ? (size_t)cut.batches * cut.splits : 0;
     return ((size_t)GATE * cut.grid + gate) * p->D * 4;
@@ -590,7 +601,8 @@ extern "C" int d2p_residual_norm_backward(const d2p_residual_norm_params* p, con
     a.dgate = dgate;
     a.lanes = team_of(p->D);
     a.by_length = Divisor(p->L);
-    const Cut cut(*p, a.lanes);
+    const Cut cut(*p, a.lanes,
+                  back_waves((dy || again) && !wide, dbias || dpost_bias, threads_of(a.lanes)));
     a.batches = cut.batches;
     a.length = cut.length;
     a.splits = cut.splits;
