@@ -113,6 +113,38 @@ def test_as_many_tokens_as_there_may_be(cuda, clean, V):
         d2p_amd.token_embedding(tokens[:, :1].expand(1, N + 1), torch.ones(V, D, device=cuda))
 
 
+def test_as_large_a_table_as_there_may_be(cuda, clean):
+    V, D, N = 2 ** 31 - 2, 8, 5000
+    weight = torch.zeros(V, D, dtype=BF16, device=cuda)
+    g = torch.Generator().manual_seed(6)
+    tokens = torch.randint(0, V, (1, N), generator=g).to(cuda)
+    tokens[0, :40] = torch.arange(40, device=cuda) % 4 + V - 4
+    tokens[0, 40:50] = 0
+    rows = torch.unique(tokens)
+    weight[rows] = torch.randn(len(rows), D, generator=g).to(BF16).to(cuda)
+    assert torch.equal(d2p_amd.token_embedding(tokens, weight), weight[tokens])
+    grad = torch.randint(-4, 5, (1, N, D), generator=g).to(BF16).to(cuda)
+    del weight
+    dw = torch.ops.d2p_amd.token_embedding_backward(grad, tokens, None, 1.0, -1, V, BF16)
+    want = torch.zeros(len(rows), D, device=cuda).index_add_(
+        0, torch.searchsorted(rows, tokens[0]), grad[0].float())
+    assert torch.equal(dw[rows].float(), want)      # whole numbers up to 40 * 4 = 160: exact
+    dw[rows] = 0
+    assert not any(bool(part.any()) for part in dw.split(1 << 27))
+
+
+def test_as_many_rows_as_there_may_be(cuda, clean):
+    N, D = 2 ** 31 - 1, 8
+    x, y = (torch.randn(1, 1, D, generator=torch.Generator().manual_seed(n)).to(BF16).to(cuda)
+            for n in range(2))
+    w = torch.ones(D, device=cuda)
+    want = d2p_amd.residual_norm(x, y, w, norm="layer")
+    got = d2p_amd.residual_norm(x.expand(1, N, D), y.expand(1, N, D), w, norm="layer")
+    for a, b in zip(got, want):
+        for part in a[0].split(1 << 28):
+            assert bool((part == b[0]).all())
+
+
 def test_more_sequences_than_a_launch_has_workgroups(cuda, clean):
     """A gate by sequence of four million sequences: each its own sum."""
     B, L, D = (1 << 22) + 77, 2, 8

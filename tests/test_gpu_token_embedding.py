@@ -86,6 +86,7 @@ CASES = [
     (5000, 1, 131072, 8, F32, F32, False, "mixed"),
     (5000, 1, 131073, 8, F32, F32, False, "falling"),
     (700, 3, 100001, 8, BF16, BF16, True, "pairs"),
+    (3, 1, 7, 1 << 20, F32, BF16, False, "mixed"),
 ]
 
 
