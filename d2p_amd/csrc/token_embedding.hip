@@ -725,7 +725,10 @@ extern "C" int d2p_token_embedding(const d2p_token_embedding_params* p, const vo
     D2P_REQUIRE(p->tokens && out && weight, "null pointer argument");
     EmbedArgs a{*p, weight, out, std::min(team_of(p->D), 64), Divisor(p->L)};
     const int most = 8 * std::max(device_cus(), 1);
-    const int grid = std::min(cdiv(p->B * p->L, 256 / a.lanes), most);
+    // a workgroup for each compute unit first, then as many rows as a team has in flight (float32 to
+    // bf16 [16384, 512]: 8.1 us, 9.3 with more workgroups of fewer rows)
+    const int rows = p->B * p->L, teams = 256 / a.lanes;
+    const int grid = std::min({cdiv(rows, teams), std::max(most / 8, cdiv(rows, DEEP * teams)), most});
     return with_pair(p->weight_dtype, p->dtype, [&](auto tw, auto to) {
         using TW = typename decltype(tw)::type;
         using TO = typename decltype(to)::type;
