@@ -35,8 +35,8 @@ struct EmbedArgs {
     Divisor by_length;
 };
 constexpr int DEEP = 4;             // rows that a team has in flight
-// As much as the card's last cache holds is written past it: bf16 [131072, 1024] of 65536 tokens 80
-// us, 103 without; with the norm that reads it next 201 either way.  Less is left for that norm:
+// As much as the card's last cache holds is written past it: bf16 [131072, 1024] of 65536 tokens
+// 80 us, 103 without; with the norm that reads it next 201 either way.  Less is left for that norm:
 // [65536, 512] 42.4 us, 44.2 past the caches.
 constexpr long long CACHES = 256 << 20;
 

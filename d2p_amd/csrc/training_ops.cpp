@@ -272,8 +272,9 @@ ThreeTensors residual_norm_forward(const Tensor& x_, const OptTensor& y_, const 
 
 using SevenTensors = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-// h: the forward's for float32, x for 16 bits and where there is no y.  dy comes back undefined where it equals dx, and
-// so does every gradient that `wanted` (bits: gate, then the four vectors) leaves out.
+// h: the forward's for float32, x for 16 bits and where there is no y.  dy comes back undefined
+// where it equals dx, and so does every gradient that `wanted` (bits: gate, then the four vectors)
+// leaves out.
 SevenTensors residual_norm_backward(const OptTensor& dh_, const OptTensor& dn_, const Tensor& h_,
                                     const OptTensor& y_, const Tensor& stats,
                                     const OptTensor& weight, const OptTensor& bias,
@@ -354,8 +355,8 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
         // y enters the gradients through its own norm, the gate's, and h where that is rounded
         const bool wide = x.scalar_type() == torch::kFloat32;
         const bool keep_y = post_norm || wants(gate) || (norm && !wide);
-        ctx->save_for_backward({given(y) && wide ? h : x, keep_y ? y.value_or(Tensor()) : Tensor(), stats,
-                                weight.value_or(Tensor()), bias.value_or(Tensor()),
+        ctx->save_for_backward({given(y) && wide ? h : x, keep_y ? y.value_or(Tensor()) : Tensor(),
+                                stats, weight.value_or(Tensor()), bias.value_or(Tensor()),
                                 post_weight.value_or(Tensor()), post_bias.value_or(Tensor()),
                                 gate.value_or(Tensor())});
         ctx->saved_data["norm"] = norm;
@@ -389,7 +390,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
                     saved(s[4]), saved(s[5]), saved(s[6]), saved(s[7]), d["norm"].toInt(),
                     d["post_norm"].toInt(), d["scale"].toDouble(), d["residual_scale"].toDouble(),
                     d["eps"].toDouble(), (at::ScalarType)d["dtype"].toInt(), block, wanted);
-                out[0] = dx;
+        out[0] = dx;
         if (block) out[1] = dy.defined() ? dy : dx;
         out[2] = dw;
         out[3] = db;
@@ -442,7 +443,6 @@ std::vector<d2p_tensor> tensor_list_of(at::TensorList ts, std::vector<Tensor>& c
     list.reserve(ts.size());
     for (const Tensor& t : ts) {
         check_on(t, ts[0], "every tensor");
-        TORCH_CHECK(t.layout() == torch::kStrided, "sparse tensors are not supported");
         const int type = type_code(t, "every tensor");
         const Tensor* from = &t;
         if (!t.is_non_overlapping_and_dense()) {

@@ -30,7 +30,8 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor,
                     padding: Optional[int] = None,
                     dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``scale`` times the rows of weight [V, D] that tokens (int32 or int64, of any shape) name:
-    [*tokens.shape, D], in ``dtype`` (weight's by default; 16 bits beside a float32 weight).
+    [*tokens.shape, D], in ``dtype`` (weight's by default; 16 bits beside a float32 weight).  D
+    is 8 at least.
 
     ``padding``: a token whose embeddings are zeros.  ``lengths`` (int32 [B], tokens [B, L]):
     positions past them are zeros too, whatever they hold.  Neither has a part in weight's
@@ -63,7 +64,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
 
     Norms are "rms" (v / sqrt(mean(v^2) + eps)), "layer" (mean taken off first) or None (z is y;
     no n).  Vectors [D] of any type are ones and zeros by default.  ``gate``: [D], [B, 1, D]
-    or [B, L, D], in float32 or y's type.  D is at most 8192.
+    or [B, L, D], in float32 or y's type.  D is from 8 to 8192.
 
     h has x's type and n has y's: the same, or 16 bits beside a float32 stream.  Without y (the
     norm before the first block) h is x, and n has ``dtype`` (x's by default).  n is formed from

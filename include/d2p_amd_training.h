@@ -105,13 +105,13 @@ int d2p_residual_norm(const d2p_residual_norm_params* p, const void* x, const vo
 /* Workspace bytes of d2p_residual_norm_backward. */
 size_t d2p_residual_norm_backward_workspace_bytes(const d2p_residual_norm_params* p);
 
-/* Gradients from dh = dL/dh and dn = dL/dn (one may be null: zeros).  stream_in, null where n has no norm or
- * no gradient: h as the forward pass wrote it if it is float32; x, with its strides, if it has 16
- * bits (h is formed from x and y again then, unrounded) or if there is no y.  y: null where it
- * is needed for neither that, nor its own norm, nor the gate's gradient.  dx, dy [B, L, D] and dgate
- * (of the gate's sizes), contiguous, in their inputs' types; dweight .. dpost_bias [D] in theirs.
- * Null: not wanted; dx, and dy where there is a y, always are, but dy may be null where it equals
- * dx (no gate, no post_norm, equal scales and types). */
+/* Gradients from dh = dL/dh and dn = dL/dn (one may be null: zeros).  stream_in, null where n has
+ * no norm or no gradient: h as the forward pass wrote it if it is float32; x, with its strides, if
+ * it has 16 bits (h is formed from x and y again then, unrounded) or if there is no y.  y: null
+ * where it is needed for neither that, nor its own norm, nor the gate's gradient.  dx, dy [B, L, D]
+ * and dgate (of the gate's sizes), contiguous, in their inputs' types; dweight .. dpost_bias [D] in
+ * theirs.  Null: not wanted; dx, and dy where there is a y, always are, but dy may be null where it
+ * equals dx (no gate, no post_norm, equal scales and types). */
 int d2p_residual_norm_backward(const d2p_residual_norm_params* p, const void* dh, const void* dn,
                                const void* stream_in, const void* y, const float* stats, void* dx,
                                void* dy, void* dgate, void* dweight, void* dbias,
