@@ -600,9 +600,11 @@ struct Plan {
         slabs = cdiv(p.D, SLAB);
         splits = 0;
         if (p.V <= SMALL && (long long)p.V * p.D <= SMALL_TABLE) {
-            // workgroups that the card's LDS holds at a time, each with more rows than its table has
-            const int groups = 256 * std::min(8, 156 / (2 * p.V));
-            splits = std::max(1, std::min(groups / slabs, N / (2 * p.V)));
+            // workgroups that the card's LDS holds at a time, but no more than rows.hip adds up as fast,
+            // each with more rows than its table has (bf16, V 4, 16384 rows, D 64 8.8 us, D 512 13.1;
+            // with eight rows and 2048 workgroups 18.1 and 22.4)
+            const int groups = 256 * std::min(4, 156 / (2 * p.V));
+            splits = std::max(1, std::min(groups / slabs, N / std::max(32, 2 * p.V)));
             if (splits > 256) splits -= splits % 256;       // as many for each compute unit
             if (N) splits = cdiv(N, cdiv(N, splits));
             total = (size_t)splits * p.V * p.D * 4;
