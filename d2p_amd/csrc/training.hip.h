@@ -128,10 +128,11 @@ inline int team_of(int D) {
 }
 
 // s / n, n a whole number below 2^24: the product with 1 / n and what it leaves, which gives
-// exact quotients exactly (a mean of equal numbers is that number).
+// exact quotients exactly (a mean of equal numbers is that number).  An infinite s leaves nothing
+// (infinity less infinity): it is infinite, so that a row whose squares overflow is normed to zeros.
 __device__ __forceinline__ float divided(float s, float n) {
-    const float per = __builtin_amdgcn_rcpf(n), q = s * per;
-    return fmaf(fmaf(-q, n, s), per, q);
+    const float per = __builtin_amdgcn_rcpf(n), q = s * per, left = fmaf(-q, n, s);
+    return __builtin_isinf(s) ? q : fmaf(left, per, q);
 }
 // 1 / sqrt(x) within two roundings, where x is below the normal numbers too
 __device__ __forceinline__ float inverse_root(float x) {
