@@ -154,6 +154,12 @@ def _residual_backward(dh, dn, h, y, stats, w, b, pw, pb, gate, norm, post, scal
               for i, v in enumerate((gate, w, b, pw, pb))))
 
 
+def _clipped(t):
+    # in the source's order where its memory is dense, which alone keeps its strides here
+    like = torch.empty_like(t)
+    return like if like.stride() == t.stride() else t.new_empty(t.shape)
+
+
 _ENCODER_FAKES.update({
     "token_embedding": lambda tokens, w, l, scale, padding, dtype: _typed(
         w, [*tokens.shape, w.size(1)], dtype),
@@ -163,7 +169,7 @@ _ENCODER_FAKES.update({
     "residual_norm_forward": _residual,
     "residual_norm_backward": _residual_backward,
     "global_norm": lambda ts: _typed(ts[0], [], torch.float32),
-    "clip_gradients": lambda ts, m: ([torch.empty_like(t) for t in ts],
+    "clip_gradients": lambda ts, m: ([_clipped(t) for t in ts],
                                      _typed(ts[0], [], torch.float32)),
     "clip_gradients_into": lambda ts, m, out: _typed(ts[0], [], torch.float32),
 })
