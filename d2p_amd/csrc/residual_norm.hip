@@ -242,12 +242,14 @@ __device__ __forceinline__ void flush(float* lds, const float* sums, float* dst,
 }
 
 // Waves a SIMD that the backward pass's registers are held to: four, but three where h is formed
-// again and the biases' sums are kept too (in workgroups of 256 threads; larger ones keep a few
-// registers in scratch).  As many workgroups as that leaves room for: fp16 [5, 1023, 333], layer norms
+// again and the biases' sums are kept too.  That is for rows within a wave; the kernels of longer
+// rows are built for workgroups of up to 1024 threads, four waves a SIMD, and there keep a few
+// registers in scratch.  As many workgroups as that leaves room for: fp16 [5, 1023, 333], layer norms
 // and a gate by token, kernel 30 -> 20 us; bf16 [131072, 512], layer and RMS norm, 200 -> 165.
+constexpr int ONE_WAVE = 256, MORE_WAVES = 1024;    // threads of a workgroup at most (MOST)
 constexpr int BACK_WAVES = 4;
-__host__ __device__ constexpr int back_waves(bool again, bool biases, int threads) {
-    return again && biases && threads == 256 ? 3 : BACK_WAVES;
+__host__ __device__ constexpr int back_waves(bool again, bool biases, int most) {
+    return again && biases && most == ONE_WAVE ? 3 : BACK_WAVES;
 }
 
 // BLOCK: y has a gradient of its own (or, in 16 bits, h is formed from it again); BIASES: some
@@ -482,13 +484,14 @@ int launch_backward(const ResidualBackArgs& a, int grid, hipStream_t st) {
                   true, st);
 }
 
+int most_threads(int D) { return D <= 64 * RUN ? ONE_WAVE : MORE_WAVES; }
 // f(rows of whole runs, threads of a workgroup at most): rows within a wave, or of several
 template <class F> int by_rows(int D, F f) {
     const auto more = [&](auto most) {
         return D % RUN ? f(std::false_type{}, most) : f(std::true_type{}, most);
     };
-    return D <= 64 * RUN ? more(std::integral_constant<int, 256>{})
-                         : more(std::integral_constant<int, 1024>{});
+    return most_threads(D) == ONE_WAVE ? more(std::integral_constant<int, ONE_WAVE>{})
+                                       : more(std::integral_constant<int, MORE_WAVES>{});
 }
 
 // How the backward pass cuts rows into segments: at most as many as the card's 256 compute units
@@ -602,7 +605,7 @@ extern "C" int d2p_residual_norm_backward(const d2p_residual_norm_params* p, con
     a.lanes = team_of(p->D);
     a.by_length = Divisor(p->L);
     const Cut cut(*p, a.lanes,
-                  back_waves((dy || again) && !wide, dbias || dpost_bias, threads_of(a.lanes)));
+                  back_waves((dy || again) && !wide, dbias || dpost_bias, most_threads(p->D)));
     a.batches = cut.batches;
     a.length = cut.length;
     a.splits = cut.splits;

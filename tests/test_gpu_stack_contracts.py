@@ -1,10 +1,13 @@
 """What the operators around the attention layers promise: layouts, memory kept, calls that a
 documented use leads to."""
+import ctypes
+
 import pytest
 import torch
 
 import d2p_amd
 from test_stack_contracts import sources
+from test_stack_host import Residual, Strides, Vector, lib  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +26,35 @@ def test_compiled_clipping_of_any_layout(cuda):
             f = torch.compile(lambda t: d2p_amd.clip_gradients([t], 2.0)[0][0].view(-1),
                               backend="aot_eager", fullgraph=True)
             assert torch.equal(f(t), eager.reshape(-1))
+
+
+@pytest.mark.parametrize("D", [513, 1024, 2048])
+def test_a_backward_pass_fills_the_card_whatever_gradients_are_wanted(cuda, lib, D):  # noqa: F811
+    """Rows of several waves: the kernel has four waves a SIMD with and without sums for the biases,
+    so as many workgroups leave parts of the vectors' gradients in the workspace."""
+    B, L = 2, 4096 + 7
+    x, y, dh, dn = (torch.randn(B, L, D, device=cuda).bfloat16() for _ in range(4))
+    w, b = torch.ones(D, device=cuda), torch.zeros(D, device=cuda)
+    stats = torch.ones(B, L, 4, device=cuda)
+    dx, dy = torch.empty_like(x), torch.empty_like(x)
+    dw, db = torch.empty_like(w), torch.empty_like(b)
+    rows = Strides(L * D, D)
+
+    def ptr(t):
+        return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+    def parts(db):
+        p = Residual(2, 2, B, L, D, 1, rows, rows, rows, rows, 2, 0, Vector(ptr(w), 0), Vector(ptr(b), 0),
+                     Vector(None, 0), Vector(None, 0), 0, None, 0, Strides(0, 0), 0.5, 1.0, 1e-5)
+        need = lib.d2p_residual_norm_backward_workspace_bytes(ctypes.byref(p))
+        ws = torch.full((need // 4,), float("nan"), device=cuda)
+        assert lib.d2p_residual_norm_backward(
+            ctypes.byref(p), ptr(dh), ptr(dn), ptr(x), ptr(y), ptr(stats), ptr(dx), ptr(dy), None,
+            ptr(dw), ptr(db), None, None, ptr(ws), need,
+            ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        torch.cuda.synchronize()
+        written = int((~ws.isnan()).sum())
+        assert written % D == 0
+        return written // D
+
+    assert parts(db) == 2 * parts(None)
