@@ -148,8 +148,9 @@ def _residual(x, y, w, b, pw, pb, gate, norm, post, scale, rscale, eps, dtype, s
 
 def _residual_backward(dh, dn, h, y, stats, w, b, pw, pb, gate, norm, post, scale, rscale, eps,
                        dtype, block, wanted):
-    same = not post and gate is None and scale == rscale and h.dtype == dtype
-    return (_contiguous(h), _typed(h, h.shape, dtype) if block and not same else None,
+    like = dh if h is None else h
+    same = not post and gate is None and scale == rscale and like.dtype == dtype
+    return (_contiguous(like), _typed(like, like.shape, dtype) if block and not same else None,
             *(_contiguous(v) if v is not None and wanted >> i & 1 else None
               for i, v in enumerate((gate, w, b, pw, pb))))
 

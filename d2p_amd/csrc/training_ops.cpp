@@ -272,48 +272,53 @@ ThreeTensors residual_norm_forward(const Tensor& x_, const OptTensor& y_, const 
 
 using SevenTensors = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
-// h: the forward's for float32, x for 16 bits and where there is no y.  dy comes back undefined
-// where it equals dx, and so does every gradient that `wanted` (bits: gate, then the four vectors)
-// leaves out.
-SevenTensors residual_norm_backward(const OptTensor& dh_, const OptTensor& dn_, const Tensor& h_,
-                                    const OptTensor& y_, const Tensor& stats,
+// h: the forward's for float32, x for 16 bits and where there is no y; needed with dn.  stats: needed
+// with a norm.  dy comes back undefined where it equals dx, and so does every gradient that `wanted`
+// (bits: gate, then the four vectors) leaves out.
+SevenTensors residual_norm_backward(const OptTensor& dh_, const OptTensor& dn_, const OptTensor& h_,
+                                    const OptTensor& y_, const OptTensor& stats,
                                     const OptTensor& weight, const OptTensor& bias,
                                     const OptTensor& post_weight, const OptTensor& post_bias,
                                     const OptTensor& gate, int64_t norm, int64_t post_norm,
                                     double scale, double residual_scale, double eps,
                                     at::ScalarType dtype, bool block, int64_t wanted) {
-    TORCH_CHECK(h_.is_cuda(), "h must be a CUDA tensor");
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(h_.device());
-    auto in = residual_inputs(h_, weight, bias, post_weight, post_bias, gate, norm, post_norm,
+    TORCH_CHECK(given(h_) || (given(dh_) && !(given(dn_) && norm)), "h is needed");
+    const Tensor& like = given(h_) ? *h_ : *dh_;    // of x's sizes and type
+    TORCH_CHECK(like.is_cuda(), "h must be a CUDA tensor");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(like.device());
+    auto in = residual_inputs(like, weight, bias, post_weight, post_bias, gate, norm, post_norm,
                               scale, residual_scale, eps, dtype);
-    const Tensor h = block && h_.scalar_type() == torch::kFloat32 ? h_.contiguous()
-                                                                  : adjacent_rows(h_);
-    in.p.x = row_strides(h);
     in.p.with_y = block;
-    Tensor dh, dn, y;
+    Tensor h, dh, dn, y;
+    if (given(h_)) {
+        h = block && h_->scalar_type() == torch::kFloat32 ? h_->contiguous() : adjacent_rows(*h_);
+        in.p.x = row_strides(h);
+    }
     if (given(dh_)) {
-        check_3d(*dh_, h, h.scalar_type(), "grad of h");
+        check_3d(*dh_, like, like.scalar_type(), "grad of h");
         dh = adjacent_rows(*dh_);
         in.p.dh = row_strides(dh);
     }
     if (given(dn_) && norm) {
-        check_3d(*dn_, h, dtype, "grad of n");
+        check_3d(*dn_, like, dtype, "grad of n");
         dn = adjacent_rows(*dn_);
         in.p.dn = row_strides(dn);
     }
     if (given(y_)) {
-        check_3d(*y_, h, dtype, "y");
+        check_3d(*y_, like, dtype, "y");
         y = adjacent_rows(*y_);
         in.p.y = row_strides(y);
     }
-    check_on(stats, h, "stats");
-    TORCH_CHECK(stats.scalar_type() == torch::kFloat32 && stats.is_contiguous() &&
-                    stats.numel() == 4 * h.size(0) * h.size(1),
-                "stats must be float32 [B, L, 4], got ", stats.sizes());
+    if (given(stats)) {
+        check_on(*stats, like, "stats");
+        TORCH_CHECK(stats->scalar_type() == torch::kFloat32 && stats->is_contiguous() &&
+                        stats->numel() == 4 * like.size(0) * like.size(1),
+                    "stats must be float32 [B, L, 4], got ", stats->sizes());
+    }
     const bool same = block && !post_norm && !given(gate) && scale == residual_scale &&
-                      h.scalar_type() == dtype;
-    Tensor dx = torch::empty(h.sizes(), h.options());
-    Tensor dy = block && !same ? torch::empty(h.sizes(), h.options().dtype(dtype)) : Tensor();
+                      like.scalar_type() == dtype;
+    Tensor dx = torch::empty(like.sizes(), like.options());
+    Tensor dy = block && !same ? torch::empty(like.sizes(), like.options().dtype(dtype)) : Tensor();
     auto of = [&](const OptTensor& v, int bit) {
         return given(v) && (wanted >> bit & 1) ? torch::empty(v->sizes(), v->options()) : Tensor();
     };
@@ -321,11 +326,12 @@ SevenTensors residual_norm_backward(const OptTensor& dh_, const OptTensor& dn_, 
            dpb = of(post_bias, 4);
     auto data = [](const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; };
     const size_t bytes = d2p_residual_norm_backward_workspace_bytes(&in.p);
-    Tensor ws = workspace(bytes, h);
+    Tensor ws = workspace(bytes, like);
     D2P_CALL(d2p_residual_norm_backward(&in.p, data(dh), data(dn), data(h), data(y),
-                                        stats.data_ptr<float>(), dx.data_ptr(), data(dy),
-                                        data(dgate), data(dw), data(db), data(dpw), data(dpb),
-                                        ws.data_ptr(), bytes, current_stream()));
+                                        given(stats) ? stats->data_ptr<float>() : nullptr,
+                                        dx.data_ptr(), data(dy), data(dgate), data(dw), data(db),
+                                        data(dpw), data(dpb), ws.data_ptr(), bytes,
+                                        current_stream()));
     return {dx, dy, dgate, dw, db, dpw, dpb};
 }
 
@@ -350,13 +356,14 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
         Tensor h, n, stats;
         std::tie(h, n, stats) =
             call_residual(x, y, weight, bias, post_weight, post_bias, gate, norm, post_norm, scale,
-                          residual_scale, eps, dtype, true);
+                          residual_scale, eps, dtype, norm || post_norm);
         auto wants = [](const OptTensor& t) { return given(t) && t->requires_grad(); };
-        // y enters the gradients through its own norm, the gate's, and h where that is rounded
+        // y enters the gradients through its own norm, the gate's, and h where that is rounded; h
+        // through its norm
         const bool wide = x.scalar_type() == torch::kFloat32;
         const bool keep_y = post_norm || wants(gate) || (norm && !wide);
-        ctx->save_for_backward({given(y) && wide ? h : x, keep_y ? y.value_or(Tensor()) : Tensor(),
-                                stats, weight.value_or(Tensor()), bias.value_or(Tensor()),
+        ctx->save_for_backward({!norm ? Tensor() : given(y) && wide ? h : x,
+                                keep_y ? y.value_or(Tensor()) : Tensor(), stats, weight.value_or(Tensor()), bias.value_or(Tensor()),
                                 post_weight.value_or(Tensor()), post_bias.value_or(Tensor()),
                                 gate.value_or(Tensor())});
         ctx->saved_data["norm"] = norm;
@@ -386,7 +393,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
         const bool block = d["block"].toBool();
         const int64_t wanted = d["wanted"].toInt();
         auto [dx, dy, dgate, dw, db, dpw, dpb] =
-            op.call(saved(grads[0]), saved(grads[1]), s[0], saved(s[1]), s[2], saved(s[3]),
+            op.call(saved(grads[0]), saved(grads[1]), saved(s[0]), saved(s[1]), saved(s[2]), saved(s[3]),
                     saved(s[4]), saved(s[5]), saved(s[6]), saved(s[7]), d["norm"].toInt(),
                     d["post_norm"].toInt(), d["scale"].toDouble(), d["residual_scale"].toDouble(),
                     d["eps"].toDouble(), (at::ScalarType)d["dtype"].toInt(), block, wanted);
@@ -621,7 +628,7 @@ TORCH_LIBRARY_FRAGMENT(d2p_amd, m) {
           ") -> (Tensor, Tensor)");
     m.def("residual_norm_forward(Tensor x, Tensor? y, " RESIDUAL_VECTORS RESIDUAL_OPTIONS
           ", bool stats) -> (Tensor, Tensor, Tensor)");
-    m.def("residual_norm_backward(Tensor? dh, Tensor? dn, Tensor h, Tensor? y, Tensor stats, "
+    m.def("residual_norm_backward(Tensor? dh, Tensor? dn, Tensor? h, Tensor? y, Tensor? stats, "
           RESIDUAL_VECTORS RESIDUAL_OPTIONS ", bool block, int wanted) -> "
           "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("global_norm(Tensor[] tensors) -> Tensor");

@@ -58,3 +58,29 @@ def test_a_backward_pass_fills_the_card_whatever_gradients_are_wanted(cuda, lib,
         return written // D
 
     assert parts(db) == 2 * parts(None)
+
+
+@pytest.mark.parametrize("types", [(torch.float32, torch.float32), (torch.float32, torch.float16),
+                                   (torch.bfloat16, torch.bfloat16)], ids=str)
+@pytest.mark.parametrize("D", [8, 9, 96, 520])
+def test_a_stream_without_norms_needs_no_stream_in_its_backward_pass(cuda, types, D):
+    """Gradients from results' gradients alone, at any alignment; x is not kept for them."""
+    g = torch.Generator().manual_seed(D)
+
+    def whole(*shape, dtype):       # numbers whose products and sums here are exact
+        return torch.randint(-4, 5, shape, generator=g).to(dtype).to(cuda)
+
+    y = whole(2, 5, D, dtype=types[1]).requires_grad_()
+    gate = whole(D, dtype=torch.float32).requires_grad_()
+    for shift in (0, 1, 3):
+        dh = whole(2 * 5 * D + shift, dtype=types[0])[shift:].view(2, 5, D)
+        for m in (None, gate):
+            x = whole(2, 5, D, dtype=types[0]).requires_grad_()
+            h, n = d2p_amd.residual_norm(x, y, norm=None, gate=m, scale=0.5, residual_scale=2.0)
+            assert n is None and torch.equal(h, (2 * x.float() + 0.5 * (1 if m is None else m) * y.float())
+                                             .to(types[0]))
+            got = torch.autograd.grad(h, [x, y] + [m] * (m is not None), dh)
+            assert torch.equal(got[0], 2 * dh)
+            assert torch.equal(got[1], (0.5 * (1 if m is None else m.detach()) * dh.float()).to(types[1]))
+            if m is not None:
+                assert torch.equal(got[2], (0.5 * dh.float() * y.detach().float()).sum((0, 1)))

@@ -24,3 +24,37 @@ def test_fakes_of_clipped_tensors_have_the_operators_strides():
         for r, (t, dense) in zip(got, ts):
             assert r.shape == t.shape
             assert r.stride() == (t.stride() if dense else torch.empty(t.shape).stride()), t.stride()
+
+
+def kept(f):
+    """The tensors that the graph of f() keeps."""
+    got = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: got.append(t) or t, lambda t: t):
+        out = f()
+    return got, out
+
+
+@pytest.mark.parametrize("types", [(torch.float32, torch.float32), (torch.float32, torch.float16),
+                                   (torch.bfloat16, torch.bfloat16)], ids=str)
+def test_a_stream_without_norms_keeps_what_its_gradients_read(types):
+    """(Meta tensors: the operators' autograd layer without their kernels.)"""
+    x, y, gate = (torch.empty(2, 5, 16, device="meta", dtype=t, requires_grad=True)
+                  for t in (types[0], types[1], types[1]))
+    op = d2p_amd.residual_norm
+    got, (h, _) = kept(lambda: op(x, y, norm=None, scale=0.5))
+    assert not got
+    dx, dy = torch.autograd.grad(h, (x, y), torch.empty_like(h))
+    assert (dx.dtype, dy.dtype) == types and dx.shape == dy.shape == x.shape
+    got, (h, _) = kept(lambda: op(x, y, norm=None, gate=gate))     # y and the gate
+    assert len(got) == 2 and all(t.shape == x.shape and t.dtype == types[1] for t in got)
+    grads = torch.autograd.grad(h, (x, y, gate), torch.empty_like(h))
+    assert [g.dtype for g in grads] == [types[0], types[1], types[1]]
+    got, (h, _) = kept(lambda: op(x, y, norm=None, gate=gate.detach()))
+    assert len(got) == 1
+    torch.autograd.grad(h, (x, y), torch.empty_like(h))
+    got, (h, _) = kept(lambda: op(x, y, norm=None, post_norm="rms"))
+    assert sorted(t.shape[-1] for t in got) == [4, 16]              # y and its norm's statistics
+    torch.autograd.grad(h, (x, y), torch.empty_like(h))
+    got, (h, n) = kept(lambda: op(x, y))
+    assert sum(t.shape == x.shape for t in got) == (1 if types[0] == torch.float32 else 2)
+    torch.autograd.grad((h, n), (x, y), (torch.empty_like(h), torch.empty_like(n)))
