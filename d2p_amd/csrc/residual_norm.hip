@@ -137,18 +137,20 @@ __global__ void __launch_bounds__(MOST) residual_norm_kernel(ResidualArgs a) {
     const int teams = blockDim.x / a.lanes;
     const unsigned rows = (unsigned)p.B * p.L;
     Vectors vec(lds + SLOTS, a.lanes);
-    const bool by_row = p.gate_kind > D2P_GATE_FEATURE;
+    // A gate by feature goes into the weight that z is made with.  Beside a bias it is taken as a
+    // row's own gate is, from one row of no stride: an infinite one times w and times b may be
+    // infinities of opposite sign, where times w v + b it is one.
+    const bool by_row = p.gate_kind > D2P_GATE_FEATURE ||
+                        (p.gate_kind == D2P_GATE_FEATURE && p.post_bias.data);
     if (p.norm != D2P_NORM_NONE) {
         vec.load(W, p.weight, 1.0f, D);
         vec.load(C, p.bias, 0.0f, D);
     }
     if (BLOCK) {
-        // what is left of a row's own gate goes into the second norm's vectors
-        const d2p_vector gate = {by_row ? nullptr : p.gate, p.gate_dtype};
         vec.load(PW, p.post_weight, 1.0f, D);
         vec.load(PC, p.post_bias, 0.0f, D);
-        vec.scale(PW, gate, p.scale, D);
-        vec.scale(PC, gate, p.scale, D);
+        vec.scale(PW, {by_row ? nullptr : p.gate, p.gate_dtype}, p.scale, D);
+        vec.scale(PC, {}, p.scale, D);
     }
     __syncthreads();
     float there[RUN];

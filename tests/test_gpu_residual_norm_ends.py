@@ -95,3 +95,37 @@ def test_sums_that_overflow(cuda):
     x[0, 1] = 1e38
     got = d2p_amd.residual_norm(x, norm="layer")[1]
     assert got[0, 1].isnan().all() and torch.equal(got[0, ::2], n[0, ::2])
+
+
+@pytest.mark.parametrize("post,bias", [(None, False), ("rms", False), ("rms", True), ("layer", False),
+                                       ("layer", True)])
+@pytest.mark.parametrize("kind", ["feature", "sequence", "token"])
+def test_infinite_gates(cuda, kind, post, bias):
+    """h as the formula in 64 bits has it: an infinite gate times z, NaN where z is 0."""
+    B, L, D = 2, 3, 24
+    for dtype, block in ((F32, F32), (F32, BF16), (BF16, BF16)):
+        x, y = rows(B, L, D, dtype, 1, cuda), rows(B, L, D, block, 2, cuda)
+        if not post:
+            y[0, 0, :6] = 0
+        w = pb = None
+        if post:
+            w = torch.linspace(-1.0, 1.0, D, device=cuda)
+            if bias:        # larger than w v, and of either sign
+                pb = 9.0 * (1 - 2 * (torch.arange(D, device=cuda) % 2)).float()
+        gate = rows(B, L, D, F32, 3, cuda)
+        gate = {"feature": gate[0, 0], "sequence": gate[:, :1], "token": gate}[kind].clone()
+        for f, value in ((1, "inf"), (2, "-inf"), (4, "nan"), (7, "inf"), (12, "inf"), (23, "-inf")):
+            gate[..., f] = float(value)
+        h, _ = d2p_amd.residual_norm(x, y, norm=None, post_norm=post, post_weight=w, post_bias=pb,
+                                     gate=gate, scale=0.5)
+        z = y.double()
+        if post:
+            z = z - z.mean(-1, keepdim=True) if post == "layer" else z
+            z = z / (z.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+            z = z if pb is None else z + pb.double()
+        want = x.double() + 0.5 * gate.double() * z
+        assert torch.equal(h.isnan(), want.isnan()), (dtype, block)
+        ends = want.isinf()
+        assert ends.any() and torch.equal(h[ends].double(), want[ends])
+        rest = ~ends & ~want.isnan()
+        assert (h[rest].double() - want[rest]).abs().max() <= (2.0 ** -7 if dtype == BF16 else 1e-4) * 20
