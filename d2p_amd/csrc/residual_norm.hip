@@ -530,6 +530,7 @@ extern "C" int d2p_residual_norm(const d2p_residual_norm_params* p, const void* 
     D2P_REQUIRE(!y == !h && !y == !p->with_y, "with_y, y and h go together");
     D2P_REQUIRE(y || (p->post_norm == D2P_NORM_NONE && p->gate_kind == D2P_GATE_NONE),
                 "a gate or a second norm needs y");
+    D2P_REQUIRE(((uintptr_t)stats & 15) == 0, "stats must be aligned to 16 bytes");
     ResidualArgs a{*p, x, y, h, n, stats, team_of(p->D), Divisor(p->L)};
     for (d2p_row_strides* s : {&a.p.x, &a.p.y}) *s = plain(*s, *p);
     a.p.gate_strides = gate_steps(*p);

@@ -7,7 +7,8 @@
  * D2P_FLOAT16, D2P_BFLOAT16): device pointers to caller-owned buffers, scratch memory from the
  * caller (*_workspace_bytes), kernels enqueued on `stream` without synchronising, 0 on success
  * and non-zero on failure with the message in d2p_last_error().  Base pointers are aligned to
- * their element.  Results do not depend on the order in which workgroups run.
+ * their element, workspaces and a residual norm's statistics are aligned to 16 bytes.  Results do
+ * not depend on the order in which workgroups run.
  */
 #ifndef D2P_AMD_TRAINING_H
 #define D2P_AMD_TRAINING_H

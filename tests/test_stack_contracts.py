@@ -1,10 +1,13 @@
 """What the operators around the attention layers promise without a GPU: layouts that a compiled
 program plans with, what a graph keeps, and refusals."""
+import ctypes
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 import d2p_amd
+from test_stack_host import FAKE, HEADER, lib, residual, said  # noqa: F401
 
 
 def sources(device):
@@ -58,3 +61,12 @@ def test_a_stream_without_norms_keeps_what_its_gradients_read(types):
     got, (h, n) = kept(lambda: op(x, y))
     assert sum(t.shape == x.shape for t in got) == (1 if types[0] == torch.float32 else 2)
     torch.autograd.grad((h, n), (x, y), (torch.empty_like(h), torch.empty_like(n)))
+
+
+def test_statistics_are_aligned_in_both_directions(lib):  # noqa: F811
+    """The forward pass writes what the backward pass reads: one rule, in the header too."""
+    p = ctypes.byref(residual())
+    for at in (0x1004, 0x1008):
+        assert lib.d2p_residual_norm(p, FAKE, FAKE, FAKE, FAKE, ctypes.c_void_p(at), None) == 1
+        assert "aligned" in said(lib)
+    assert "aligned to 16 bytes" in open(HEADER).read()
