@@ -217,6 +217,16 @@ class SequenceAttention(nn.Module):
             raise ValueError(f"a cache of {room} tokens exceeds the layer's max_length "
                              f"{self.cos.shape[0]}")
 
+    def _check_step(self, batch, n, cache):
+        if not self.causal:
+            raise ValueError("step() needs a causal layer")
+        there, room = cache.keys.shape[:2]
+        if batch != there:
+            raise ValueError(f"{batch} sequences beside a cache of {there}")
+        if n > room:
+            raise ValueError(f"{n} tokens do not fit a cache of {room}")
+        self._check_room(room)
+
     def new_cache(self, batch: int, max_length: int, dtype=None) -> KeyValueCache:
         self._check_room(max_length)
         like = self.qkv.weight
@@ -231,12 +241,8 @@ class SequenceAttention(nn.Module):
         whose lengths grow by n, and each attends to all before it.  The host does not know
         the lengths, so nothing waits: a sequence that outgrows its cache comes back NaN, in
         that call and all later ones, and so does one whose length is below zero."""
-        if not self.causal:
-            raise ValueError("step() needs a causal layer")
+        self._check_step(x.shape[0], x.shape[1], cache)
         n, room = x.shape[1], cache.keys.shape[1]
-        if n > room:
-            raise ValueError(f"{n} tokens do not fit a cache of {room}")
-        self._check_room(room)
         at = cache.lengths[:, None] + torch.arange(n, dtype=torch.int32, device=x.device)
         q, k, v = self._project(x, at)
         where = at.long().clamp(0, room - 1)[:, :, None, None].expand_as(k)

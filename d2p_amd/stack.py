@@ -198,5 +198,12 @@ class SequenceEncoder(nn.Module):
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, caches: Sequence[KeyValueCache]) -> torch.Tensor:
-        """New tokens [B, n] of each sequence; see ``SequenceAttention.step``."""
+        """New tokens [B, n] of each sequence, caches from ``new_caches``; see
+        ``SequenceAttention.step``.  A call that is refused leaves all caches as they are."""
+        if len(caches) != len(self.layers):
+            raise ValueError(f"need a cache for each of {len(self.layers)} layers, got {len(caches)}")
+        if tokens.dim() != 2:
+            raise ValueError(f"tokens must be [B, n], got {tuple(tokens.shape)}")
+        for layer, cache in zip(self.layers, caches):
+            layer._check_step(*tokens.shape, cache)
         return self._run(tokens, None, lambda i, layer, n: layer.step(n, caches[i]))

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import d2p_amd
-from test_stack_contracts import sources
+from test_stack_contracts import caches_that_do_not_fit, sources
 from test_stack_host import Residual, Strides, Vector, lib  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -84,3 +84,11 @@ def test_a_stream_without_norms_needs_no_stream_in_its_backward_pass(cuda, types
             assert torch.equal(got[1], (0.5 * (1 if m is None else m.detach()) * dh.float()).to(types[1]))
             if m is not None:
                 assert torch.equal(got[2], (0.5 * dh.float() * y.detach().float()).sum((0, 1)))
+
+
+def test_a_refused_step_leaves_the_caches(cuda):
+    m = d2p_amd.SequenceEncoder(5, 16, 2, 2, causal=True).to(cuda)
+    for n, caches, match in caches_that_do_not_fit(m):
+        with pytest.raises(ValueError, match=match):
+            m.step(torch.zeros(2, n, dtype=torch.int64, device=cuda), caches)
+        assert not any(t.any() for c in caches for t in c)

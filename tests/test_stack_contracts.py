@@ -70,3 +70,24 @@ def test_statistics_are_aligned_in_both_directions(lib):  # noqa: F811
         assert lib.d2p_residual_norm(p, FAKE, FAKE, FAKE, FAKE, ctypes.c_void_p(at), None) == 1
         assert "aligned" in said(lib)
     assert "aligned to 16 bytes" in open(HEADER).read()
+
+
+def caches_that_do_not_fit(m, batch=2):
+    """(tokens that come, caches, what is said)"""
+    good = m.new_caches(batch, 8)
+    return ((3, good[:1], "cache for each"), (3, good + good[:1], "cache for each"), (3, [], "cache for each"),
+            (3, good[:1] + [m.layers[1].new_cache(batch, 2)], "do not fit"),
+            (3, good[:1] + [m.layers[1].new_cache(batch + 1, 8)], "sequences"),
+            (9, good, "do not fit"))
+
+
+def test_steps_check_every_cache_first():
+    m = d2p_amd.SequenceEncoder(5, 16, 2, 2, causal=True)
+    for n, caches, match in caches_that_do_not_fit(m):
+        with pytest.raises(ValueError, match=match):
+            m.step(torch.zeros(2, n, dtype=torch.int64), caches)
+    with pytest.raises(ValueError, match="tokens must"):
+        m.step(torch.zeros(2, dtype=torch.int64), m.new_caches(2, 8))
+    with pytest.raises(ValueError, match="causal"):
+        m = d2p_amd.SequenceEncoder(5, 16, 2, 2)
+        m.step(torch.zeros(2, 1, dtype=torch.int64), m.new_caches(2, 8))
