@@ -180,8 +180,11 @@ class SequenceEncoder(nn.Module):
         x, n = residual_norm(x, None, self.weights[0], at(self.biases, 0), norm=self.norm,
                              eps=self.eps, dtype=kind if x.dtype == torch.float32 else None)
         for i, layer in enumerate(self.layers):
+            y = attend(i, layer, n)
+            if x.dtype != torch.float32:
+                y = y.to(x.dtype)       # (a 16-bit stream under autocast to the other 16 bits)
             x, n = residual_norm(
-                x, attend(i, layer, n), self.weights[i + 1], at(self.biases, i + 1), norm=self.norm,
+                x, y, self.weights[i + 1], at(self.biases, i + 1), norm=self.norm,
                 post_norm=self.post_norm, post_weight=at(self.post_weights, i),
                 post_bias=at(self.post_biases, i), gate=at(self.gates, i), eps=self.eps)
         return n

@@ -92,3 +92,23 @@ def test_a_refused_step_leaves_the_caches(cuda):
         with pytest.raises(ValueError, match=match):
             m.step(torch.zeros(2, n, dtype=torch.int64, device=cuda), caches)
         assert not any(t.any() for c in caches for t in c)
+
+
+@pytest.mark.parametrize("dtype,other", [(torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16)])
+def test_a_16_bit_encoder_under_autocast_to_the_other_16_bits(cuda, dtype, other):
+    """The stream keeps its type, the blocks run in autocast's: within 30 roundings of bfloat16, the
+    coarser of the two, of the encoder in 32 bits."""
+    torch.manual_seed(0)
+    m = d2p_amd.SequenceEncoder(23, 64, 4, 3, 2, causal=True, post_norm="rms", gated=0.3).to(cuda).eval()
+    tokens = torch.randint(0, 23, (3, 40), device=cuda)
+    want = m(tokens)
+    m = m.to(dtype)
+    with torch.autocast("cuda", dtype=other):
+        got = m(tokens)
+        got.float().square().sum().backward()
+        caches = m.new_caches(3, 40)
+        steps = torch.cat([m.step(tokens[:, a:b], caches) for a, b in ((0, 9), (9, 10), (10, 40))], 1)
+    assert got.dtype == steps.dtype == dtype
+    assert all(p.grad.dtype == dtype and p.grad.isfinite().all() for p in m.parameters())
+    for out in (got, steps):
+        assert (out - want).abs().max() <= 30 * 2.0 ** -8 * want.abs().max()
