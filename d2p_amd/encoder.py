@@ -131,6 +131,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                        float(dropout), key, key_tensor)
 
 
+def _lengths32(lengths: torch.Tensor) -> torch.Tensor:
+    """Lengths in 32 bits; those of 64 that do not fit stay wrong ones."""
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(-1, 2 ** 31 - 1)
+    return lengths.to(torch.int32)
+
+
 class KeyValueCache(NamedTuple):
     """Keys and values [B, max length, Hkv, D] of the tokens seen so far, and how many there
     are of each sequence (int32 [B])."""
@@ -201,11 +208,11 @@ class SequenceAttention(nn.Module):
 
     def forward(self, x: torch.Tensor, lengths: Optional[torch.Tensor] = None,
                 seed: Union[int, torch.Tensor, None] = None) -> torch.Tensor:
-        """x [B, L, dim], lengths int32 [B]; a dropping layer in training draws its seed from
+        """x [B, L, dim], lengths int32 or int64 [B]; a dropping layer in training draws its seed from
         torch's generator unless it is given one."""
         q, k, v = self._project(x, None)
         if lengths is not None:
-            lengths = lengths.to(torch.int32)[:, None].expand(-1, 2).contiguous()
+            lengths = _lengths32(lengths)[:, None].expand(-1, 2).contiguous()
         p = self.dropout if self.training else 0.0
         if p and seed is None:
             seed = torch.randint(-2 ** 63, 2 ** 63 - 1, (1,), device=x.device)

@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from . import _ops  # noqa: F401  (loads the operator library)
-from .encoder import KeyValueCache, SequenceAttention
+from .encoder import KeyValueCache, SequenceAttention, _lengths32
 
 _NORMS = {None: 0, "rms": 1, "layer": 2}
 
@@ -190,10 +190,10 @@ class SequenceEncoder(nn.Module):
         return n
 
     def forward(self, tokens: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """tokens [B, L], lengths int32 [B]; a dropping encoder in training draws its seeds from
+        """tokens [B, L], lengths int32 or int64 [B]; a dropping encoder in training draws its seeds from
         torch's generator."""
         if lengths is not None:
-            lengths = lengths.to(torch.int32)
+            lengths = _lengths32(lengths)
         return self._run(tokens, lengths, lambda i, layer, n: layer(n, lengths))
 
     def new_caches(self, batch: int, max_length: int, dtype=None) -> List[KeyValueCache]:

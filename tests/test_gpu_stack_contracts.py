@@ -112,3 +112,13 @@ def test_a_16_bit_encoder_under_autocast_to_the_other_16_bits(cuda, dtype, other
     assert all(p.grad.dtype == dtype and p.grad.isfinite().all() for p in m.parameters())
     for out in (got, steps):
         assert (out - want).abs().max() <= 30 * 2.0 ** -8 * want.abs().max()
+
+
+def test_lengths_that_pass_32_bits_are_wrong_ones(cuda):
+    """They come back NaN as other lengths out of range do, in the layer and in the encoder."""
+    m = d2p_amd.SequenceEncoder(23, 64, 4, 2).to(cuda)
+    tokens = torch.randint(0, 23, (4, 12), device=cuda)
+    lengths = torch.tensor([12, 2 ** 32 + 12, -2 ** 32 + 5, 7], device=cuda)
+    for out in (m(tokens, lengths), m.layers[0](torch.randn(4, 12, 64, device=cuda), lengths)):
+        assert out[1:3].isnan().all() and out[::3].isfinite().all()
+    assert torch.equal(m(tokens, lengths)[::3], m(tokens, lengths.clamp(0, 12).int())[::3])
