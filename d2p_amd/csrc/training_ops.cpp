@@ -7,6 +7,8 @@
 // differentiate, and the operators that do their work go through the dispatcher.
 #include "encoder_util.h"
 
+#include <ATen/MemoryOverlap.h>
+
 #include <cmath>
 #include <tuple>
 #include <vector>
@@ -527,8 +529,8 @@ std::tuple<std::vector<Tensor>, Tensor> clip_gradients(at::TensorList ts, double
 }
 
 // Results that share memory with each other, or with a source other than their own, would be
-// read after they are written.
-void check_apart(const std::vector<d2p_tensor>& list) {
+// read after they are written.  `more`: results that are written later, from memory of their own.
+void check_apart(const std::vector<d2p_tensor>& list, const std::vector<d2p_tensor>& more) {
     using Range = std::pair<uintptr_t, uintptr_t>;
     auto range = [](const void* from, const d2p_tensor& t) {
         return Range((uintptr_t)from, (uintptr_t)from + t.n * (t.dtype == D2P_FLOAT32 ? 4 : 2));
@@ -548,6 +550,12 @@ void check_apart(const std::vector<d2p_tensor>& list) {
                                    [](uintptr_t x, const Range& y) { return x < y.second; });
         apart &= it == results.end() || it->first >= r.second;
     }
+    if (!more.empty()) {        // (the sources have all been read by then)
+        for (const auto& t : more)
+            if (t.n) results.push_back(range(t.dst, t));
+        std::sort(results.begin(), results.end());
+        for (size_t i = 1; i < results.size(); ++i) apart &= results[i - 1].second <= results[i].first;
+    }
     TORCH_CHECK(apart, "tensors share memory that a result is written to");
 }
 
@@ -556,10 +564,12 @@ Tensor clip_gradients_into(at::TensorList ts, double max_norm, at::TensorList ou
     TORCH_CHECK(ts[0].is_cuda(), "every tensor must be a CUDA tensor");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(ts[0].device());
     TORCH_CHECK(out.size() == ts.size(), "out must have ", ts.size(), " tensors, got ", out.size());
-    std::vector<Tensor> copies, apart;
+    std::vector<Tensor> copies;
     copies.reserve(ts.size());
     auto list = tensor_list_of(ts, copies);
-    std::vector<std::pair<size_t, Tensor>> late;    // results that are no dense memory
+    // results in another order than their source's, or in no dense memory; those that are dense
+    std::vector<std::pair<size_t, Tensor>> late;
+    std::vector<d2p_tensor> late_dense;
     for (size_t i = 0; i < list.size(); ++i) {
         check_on(out[i], ts[0], "every tensor of out");
         TORCH_CHECK(out[i].sizes() == ts[i].sizes() && out[i].scalar_type() == ts[i].scalar_type(),
@@ -569,13 +579,16 @@ Tensor clip_gradients_into(at::TensorList ts, double max_norm, at::TensorList ou
         if (dense ? out[i].strides() == ts[i].strides() : out[i].is_contiguous()) {
             list[i].dst = out[i].data_ptr();
         } else {
+            at::assert_no_internal_overlap(out[i]);
+            if (out[i].is_non_overlapping_and_dense())
+                late_dense.push_back({nullptr, out[i].data_ptr(), list[i].n, list[i].dtype});
             late.emplace_back(i, dense ? torch::empty_strided(ts[i].sizes(), ts[i].strides(),
                                                               ts[i].options())
                                        : torch::empty(ts[i].sizes(), ts[i].options()));
             list[i].dst = late.back().second.data_ptr();
         }
     }
-    check_apart(list);
+    check_apart(list, late_dense);
     Tensor norm = clip_lists(list, ts[0], max_norm);
     for (auto& [i, t] : late) out[i].copy_(t);
     return norm;

@@ -122,3 +122,35 @@ def test_lengths_that_pass_32_bits_are_wrong_ones(cuda):
     for out in (m(tokens, lengths), m.layers[0](torch.randn(4, 12, 64, device=cuda), lengths)):
         assert out[1:3].isnan().all() and out[::3].isfinite().all()
     assert torch.equal(m(tokens, lengths)[::3], m(tokens, lengths.clamp(0, 12).int())[::3])
+
+
+def test_results_in_another_order_share_no_memory_either(cuda):
+    """Refused before anything is written, as results in their source's order are."""
+    op = d2p_amd.clip_gradients
+    base = torch.zeros(64, device=cuda)
+    x, y = torch.ones(6, 5, device=cuda), torch.ones(10, device=cuda)
+    turned = base[:30].view(5, 6).t()
+    for out in ([turned, base[29:39]], [turned, base[:10]], [turned, y[:1].expand(10)]):
+        with pytest.raises(RuntimeError, match="share|single memory"):
+            op([x, y], 1.0, out=out)
+        with pytest.raises(RuntimeError, match="share|single memory"):
+            op([y, x], 1.0, out=out[::-1])
+    with pytest.raises(RuntimeError, match="share"):
+        op([x, x.clone()], 1.0, out=[turned, base[:30].view(5, 6).t()])
+    # a gradient that is broadcast: the others are not clipped when it is refused
+    p, q = (torch.nn.Parameter(torch.zeros(4, 4, device=cuda)) for _ in range(2))
+    p.grad, q.grad = torch.ones(4, 4, device=cuda), torch.ones(1, 1, device=cuda).expand(4, 4)
+    with pytest.raises(RuntimeError, match="single memory"):
+        d2p_amd.clip_grad_norm_([p, q], 1.0)
+    assert not base.any() and (p.grad == 1).all() and (x == 1).all() and (y == 1).all()
+    # what stays apart is written: neighbours, columns of one buffer, a source's own memory turned
+    want, _ = op([x, y], 1.0)
+    op([x, y], 1.0, out=[turned, base[30:40]])
+    assert torch.equal(turned, want[0]) and torch.equal(base[30:40], want[1]) and not base[40:].any()
+    columns = torch.zeros(10, 2, device=cuda)
+    got, _ = op([y, 2 * y], 1.0, out=[columns[:, 0], columns[:, 1]])
+    assert torch.equal(columns[:, 1], 2 * columns[:, 0]) and columns.all()
+    a = torch.arange(16.0, device=cuda).view(4, 4)
+    want, _ = op([a.t()], 1.0)
+    op([a.t()], 1.0, out=[a])
+    assert torch.equal(a, want[0])
