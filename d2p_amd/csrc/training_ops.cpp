@@ -378,7 +378,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
         ctx->saved_data["wanted"] = int64_t(wants(gate)) | wants(weight) << 1 | wants(bias) << 2 |
                                     wants(post_weight) << 3 | wants(post_bias) << 4;
         ctx->set_materialize_grads(false);
-        // (a function's results are tensors)
+        // (a function's results are tensors; residual_norm_autograd leaves these out)
         for (Tensor* t : {&h, &n})
             if (!t->defined()) *t = torch::empty({0}, x.options());
         return {h, n};
@@ -433,7 +433,7 @@ std::tuple<Tensor, Tensor> residual_norm_autograd(
     if (differentiates({&x, &t[0], &t[1], &t[2], &t[3], &t[4], &t[5]})) {
         auto r = ResidualNormFunction::apply(x, y, weight, bias, post_weight, post_bias, gate, norm,
                                              post_norm, scale, residual_scale, eps, dtype);
-        return {r[0], r[1]};
+        return {given(y) ? r[0] : Tensor(), norm ? r[1] : Tensor()};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     auto [h, n, stats] = call_residual(x, y, weight, bias, post_weight, post_bias, gate, norm,

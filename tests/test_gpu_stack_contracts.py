@@ -154,3 +154,22 @@ def test_results_in_another_order_share_no_memory_either(cuda):
     want, _ = op([a.t()], 1.0)
     op([a.t()], 1.0, out=[a])
     assert torch.equal(a, want[0])
+
+
+def test_operators_registrations_agree(cuda):
+    """Schemas, fakes, autograd and compiled programs, as torch's own check has it.  (Clipped results
+    share one buffer, which that check does not allow.)"""
+    o = torch.ops.d2p_amd
+    t = torch.randint(0, 9, (3, 7), device=cuda)
+    w = torch.randn(9, 16, device=cuda, requires_grad=True)
+    lengths = torch.tensor([7, 2, 0], dtype=torch.int32, device=cuda)
+    x, y = (torch.randn(3, 7, 16, device=cuda, requires_grad=True) for _ in range(2))
+    v = torch.randn(16, device=cuda, requires_grad=True)
+    ts = [torch.randn(5, device=cuda), torch.randn(4, 6, device=cuda).t(), torch.randn(4, 6, device=cuda)[:, ::2]]
+    into = [torch.empty(a.shape, device=cuda) for a in ts]
+    for op, args in ((o.token_embedding, (t, w, lengths, 2.0, 3, torch.float16)),
+                     (o.residual_norm, (x, y, v, v, v, v, v, 2, 2, 0.5, 1.0, 1e-6, torch.float32)),
+                     (o.residual_norm, (x, y, *[None] * 5, 0, 0, 0.5, 1.0, 1e-6, torch.float32)),
+                     (o.residual_norm, (x, None, v, *[None] * 4, 1, 0, 1.0, 1.0, 1e-6, torch.bfloat16)),
+                     (o.global_norm, (ts,)), (o.clip_gradients_into, (ts, 1.0, into))):
+        torch.library.opcheck(op.default, args)

@@ -91,3 +91,18 @@ def test_steps_check_every_cache_first():
     with pytest.raises(ValueError, match="causal"):
         m = d2p_amd.SequenceEncoder(5, 16, 2, 2)
         m.step(torch.zeros(2, 1, dtype=torch.int64), m.new_caches(2, 8))
+
+
+def test_the_operator_gives_no_result_that_is_not_there():
+    """None in its place, with gradients as without: not a tensor of no numbers that a program could
+    take a gradient of.  (Meta tensors: the operators' autograd layer without their kernels.)"""
+    op = torch.ops.d2p_amd.residual_norm
+    x, y = (torch.empty(2, 5, 16, device="meta", requires_grad=True) for _ in range(2))
+    first = (None, None, None, None, None, None, 1, 0, 1.0, 1.0, 1e-6, torch.float32)
+    plain = (None, None, None, None, None, 0, 0, 1.0, 1.0, 1e-6, torch.float32)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad):
+            h, n = op(x, *first)
+            assert h is None and n.shape == x.shape and n.requires_grad == grad
+            h, n = op(x, y, *plain)
+            assert n is None and h.shape == x.shape and h.requires_grad == grad
