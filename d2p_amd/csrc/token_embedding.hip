@@ -3,8 +3,9 @@
 //
 // Forward: bound by reading rows and writing the result; a team of lanes copies rows, eight
 // numbers a lane, four rows in flight (two: 42 us for 38 at [262144, 256] of 30000, eight 44), in up
-// to eight workgroups a compute unit (as many as there are rows: 67).  bf16 [131072, 1024] of 65536
-// tokens in 80 us: 3.4 TB/s written, about 5 with what is read.
+// to eight workgroups a compute unit (as many as there are rows: 67).  (Of 30000 some of which are
+// frequent; of as many that all occur alike 44 us.)  bf16 [131072, 1024] of 65536 tokens in 80 us:
+// 3.4 TB/s written, about 5 with what is read.
 //
 // Backward: the gradient's rows of one token have to come together.  Positions are sorted by
 // token (a stable radix sort of up to ten bits a pass, so that sums have one order), cut into chunks

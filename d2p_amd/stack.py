@@ -68,7 +68,8 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None,
 
     h has x's type and n has y's: the same, or 16 bits beside a float32 stream.  Without y (the
     norm before the first block) h is x, and n has ``dtype`` (x's by default).  n is formed from
-    h before h is rounded.  Gradients flow to all tensors.
+    h before h is rounded.  A row whose squares (a layer norm's: around its mean) pass float32 is
+    normed to zeros.  Gradients flow to all tensors.
     """
     if y is None:
         if post_norm is not None or gate is not None or residual_scale != 1.0:
@@ -108,8 +109,8 @@ def clip_gradients(tensors: Sequence[torch.Tensor], max_norm: float,
     ``max_norm``, as they are otherwise.  Nothing waits for the device.
 
     Results go to ``out`` if it is given: tensors of the same shapes and types, which may be
-    the sources themselves but may not share memory otherwise.  An infinite norm scales by
-    zero, a NaN makes all results NaN.
+    the sources themselves but may not share memory otherwise.  New ones share one buffer.  An
+    infinite norm scales by zero, a NaN makes all results NaN.
     """
     tensors = _some(tensors)
     if out is None:
@@ -126,7 +127,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]],
                     max_norm: float) -> torch.Tensor:
     """Clips the gradients of ``parameters`` in place to a common 2-norm of ``max_norm`` at most,
     and returns the norm that they had (float32, on the device).  Parameters without a gradient
-    are left out, one that is listed twice counts once."""
+    are left out, one that is listed twice counts once.  The factor is max_norm / norm; torch's
+    function of this name divides by norm + 1e-6."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = {id(p.grad): p.grad for p in parameters if p.grad is not None}
     if not grads:

@@ -65,7 +65,8 @@ int d2p_token_embedding_backward(const d2p_token_embedding_params* p, const void
  *   N(v; w, b) = w v / sqrt(mean(v^2) + eps) + b                       (D2P_NORM_RMS)
  *              = w (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) + b   (D2P_NORM_LAYER)
  * n is formed from h before h is rounded to its type.  Without y: h = x, and only n is
- * written. */
+ * written.  All is computed in float32: a row whose sum of squares (a layer norm's: around its
+ * mean) is infinite there has N = b. */
 #define D2P_NORM_NONE 0
 #define D2P_NORM_RMS 1
 #define D2P_NORM_LAYER 2
