@@ -365,7 +365,8 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
         const bool wide = x.scalar_type() == torch::kFloat32;
         const bool keep_y = post_norm || wants(gate) || (norm && !wide);
         ctx->save_for_backward({!norm ? Tensor() : given(y) && wide ? h : x,
-                                keep_y ? y.value_or(Tensor()) : Tensor(), stats, weight.value_or(Tensor()), bias.value_or(Tensor()),
+                                keep_y ? y.value_or(Tensor()) : Tensor(), stats,
+                                weight.value_or(Tensor()), bias.value_or(Tensor()),
                                 post_weight.value_or(Tensor()), post_bias.value_or(Tensor()),
                                 gate.value_or(Tensor())});
         ctx->saved_data["norm"] = norm;
@@ -395,8 +396,8 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
         const bool block = d["block"].toBool();
         const int64_t wanted = d["wanted"].toInt();
         auto [dx, dy, dgate, dw, db, dpw, dpb] =
-            op.call(saved(grads[0]), saved(grads[1]), saved(s[0]), saved(s[1]), saved(s[2]), saved(s[3]),
-                    saved(s[4]), saved(s[5]), saved(s[6]), saved(s[7]), d["norm"].toInt(),
+            op.call(saved(grads[0]), saved(grads[1]), saved(s[0]), saved(s[1]), saved(s[2]),
+                    saved(s[3]), saved(s[4]), saved(s[5]), saved(s[6]), saved(s[7]), d["norm"].toInt(),
                     d["post_norm"].toInt(), d["scale"].toDouble(), d["residual_scale"].toDouble(),
                     d["eps"].toDouble(), (at::ScalarType)d["dtype"].toInt(), block, wanted);
         out[0] = dx;
@@ -579,7 +580,7 @@ Tensor clip_gradients_into(at::TensorList ts, double max_norm, at::TensorList ou
         if (dense ? out[i].strides() == ts[i].strides() : out[i].is_contiguous()) {
             list[i].dst = out[i].data_ptr();
         } else {
-            at::assert_no_internal_overlap(out[i]);
+            if (list[i].n) at::assert_no_internal_overlap(out[i]);
             if (out[i].is_non_overlapping_and_dense())
                 late_dense.push_back({nullptr, out[i].data_ptr(), list[i].n, list[i].dtype});
             late.emplace_back(i, dense ? torch::empty_strided(ts[i].sizes(), ts[i].strides(),

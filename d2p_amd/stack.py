@@ -192,8 +192,8 @@ class SequenceEncoder(nn.Module):
         return n
 
     def forward(self, tokens: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """tokens [B, L], lengths int32 or int64 [B]; a dropping encoder in training draws its seeds from
-        torch's generator."""
+        """tokens [B, L], lengths int32 or int64 [B]; a dropping encoder in training draws its seeds
+        from torch's generator."""
         if lengths is not None:
             lengths = _lengths32(lengths)
         return self._run(tokens, lengths, lambda i, layer, n: layer(n, lengths))
@@ -205,7 +205,7 @@ class SequenceEncoder(nn.Module):
     def step(self, tokens: torch.Tensor, caches: Sequence[KeyValueCache]) -> torch.Tensor:
         """New tokens [B, n] of each sequence, caches from ``new_caches``; see
         ``SequenceAttention.step``.  A call that is refused leaves all caches as they are."""
-        if len(caches) != len(self.layers):
+        if len(caches) < len(self.layers):
             raise ValueError(f"need a cache for each of {len(self.layers)} layers, got {len(caches)}")
         if tokens.dim() != 2:
             raise ValueError(f"tokens must be [B, n], got {tuple(tokens.shape)}")

@@ -92,6 +92,9 @@ def test_a_refused_step_leaves_the_caches(cuda):
         with pytest.raises(ValueError, match=match):
             m.step(torch.zeros(2, n, dtype=torch.int64, device=cuda), caches)
         assert not any(t.any() for c in caches for t in c)
+    caches = m.new_caches(2, 8) + m.new_caches(2, 8)        # more than there are layers
+    m.step(torch.zeros(2, 1, dtype=torch.int64, device=cuda), caches)
+    assert [int(c.lengths[0]) for c in caches] == [1, 1, 0, 0]
 
 
 @pytest.mark.parametrize("dtype,other", [(torch.float16, torch.bfloat16), (torch.bfloat16, torch.float16)])
@@ -150,6 +153,8 @@ def test_results_in_another_order_share_no_memory_either(cuda):
     columns = torch.zeros(10, 2, device=cuda)
     got, _ = op([y, 2 * y], 1.0, out=[columns[:, 0], columns[:, 1]])
     assert torch.equal(columns[:, 1], 2 * columns[:, 0]) and columns.all()
+    empty = torch.ones(1, 1, device=cuda).expand(4, 4)[:0]      # of no numbers: nothing is written
+    op([empty, y], 1.0, out=[empty, base[30:40]])
     a = torch.arange(16.0, device=cuda).view(4, 4)
     want, _ = op([a.t()], 1.0)
     op([a.t()], 1.0, out=[a])
@@ -165,7 +170,8 @@ def test_operators_registrations_agree(cuda):
     lengths = torch.tensor([7, 2, 0], dtype=torch.int32, device=cuda)
     x, y = (torch.randn(3, 7, 16, device=cuda, requires_grad=True) for _ in range(2))
     v = torch.randn(16, device=cuda, requires_grad=True)
-    ts = [torch.randn(5, device=cuda), torch.randn(4, 6, device=cuda).t(), torch.randn(4, 6, device=cuda)[:, ::2]]
+    ts = [torch.randn(5, device=cuda), torch.randn(4, 6, device=cuda).t(),
+          torch.randn(4, 6, device=cuda)[:, ::2]]
     into = [torch.empty(a.shape, device=cuda) for a in ts]
     for op, args in ((o.token_embedding, (t, w, lengths, 2.0, 3, torch.float16)),
                      (o.residual_norm, (x, y, v, v, v, v, v, 2, 2, 0.5, 1.0, 1e-6, torch.float32)),
