@@ -179,3 +179,12 @@ def test_operators_registrations_agree(cuda):
                      (o.residual_norm, (x, None, v, *[None] * 4, 1, 0, 1.0, 1.0, 1e-6, torch.bfloat16)),
                      (o.global_norm, (ts,)), (o.clip_gradients_into, (ts, 1.0, into))):
         torch.library.opcheck(op.default, args)
+
+
+def test_second_derivative_without_norms_raises(cuda):
+    x, y = (torch.randn(2, 5, 32, device=cuda, requires_grad=True) for _ in range(2))
+    g = torch.randn(2, 5, 32, device=cuda, requires_grad=True)
+    h, _ = d2p_amd.residual_norm(x, y, norm=None, scale=0.5)
+    d = torch.autograd.grad(h, (x, y), g, create_graph=True)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        d[1].sum().backward()
